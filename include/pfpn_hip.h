@@ -220,6 +220,58 @@ int pfpn_resample(float* loc, float* logstd, float* bias, float* weight, int H,
                   const float* u_noise, int A, int N, float threshold, int tanh_mode, int topk, float fixed_sigma,
                   int32_t* dead_out, int32_t* src_out, void* stream);
 
+/* ---- policy objectives -------------------------------------------------------------------- */
+/* Categorical logits of these entry points: [B, A, N] of element type `dtype` (0 float32, 1 bfloat16, 2 float16), one row every
+ * `row_stride` elements (>= A*N: a padded row), the [A, N] part of a row dense; any alignment of the element type.  A = 1: one
+ * choice of N per row (a token of a vocabulary).  A <= 4096, N <= 2^30.  `index` [B, A]: int32, or int64 with index64 != 0; an
+ * index outside [0, N) takes its choice out of the row (log-prob 0, zero gradient).  A logit of -inf closes a category; a segment
+ * with every category closed has log-prob -inf and a zero gradient.  Gradients have the logits' type, one rounding from 32 bits;
+ * dlogits must not overlap logits.  Workspaces need no initialisation; results are bitwise reproducible. */
+size_t pfpn_categorical_workspace_bytes(int B, int A, int N);
+/* logp[b] = sum_a log softmax(logits[b,a,:])[index[b,a]] -- the log-prob of the categories a policy drew (the index draw:
+ * reference networks/utils.py:187-194). */
+int pfpn_categorical_logprob_fwd(const void* logits, int dtype, long long row_stride, const void* index, int index64,
+                                 int B, int A, int N, float* logp, void* workspace, size_t workspace_bytes, void* stream);
+/* dlogits[b,a,n] (+)= dlogp[b] (1[n = index] - softmax_n); a row with dlogp 0 is not read. */
+int pfpn_categorical_logprob_bwd(const void* logits, int dtype, long long row_stride, const void* index, int index64,
+                                 const float* dlogp, int B, int A, int N, int accumulate, void* dlogits,
+                                 long long grad_stride, void* workspace, size_t workspace_bytes, void* stream);
+/* Clipped policy loss with a KL term, forward and backward from the logits (the clipped surrogate of reference ppo.py:44-54 on
+ * categorical log-probs, plus the sampled KL term to a reference policy):
+ *   a = clip((adv - mean) rstd) (adv_stats NULL: adv itself), r = exp(logp - logp_old), d = logp_ref - logp,
+ *   loss = sum_b w_b (-min(r a, clip(r, 1 - clip_eps_low, 1 + clip_eps_high) a) + kl_coef (exp(d) - 1 - d)).
+ * logp_ref optional (NULL: no KL term, kl_coef must be 0); weight [B] optional (NULL: 1/B each) -- a row of weight 0 is not read
+ * (whatever it holds), its logp and gradient are 0.  loss4 = {loss, sum w policy term, sum w kl, sum of w where the clip binds}. */
+int pfpn_categorical_ppo_fwd_bwd(const void* logits, int dtype, long long row_stride, const void* index, int index64,
+                                 const float* logp_old, const float* adv, const float* logp_ref, const float* weight,
+                                 const float* adv_stats, int B, int A, int N, double clip_eps_low, double clip_eps_high,
+                                 double kl_coef, float* logp, void* dlogits, long long grad_stride, float* loss4,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+/* The same loss on n log-probs from elsewhere (pfpn_logprob_fwd's): dlogp [n], loss4; pfpn_logprob_bwd carries dlogp on. */
+size_t pfpn_policy_kl_workspace_bytes(long long n);
+int pfpn_policy_kl_loss(const float* logp, const float* logp_old, const float* adv, const float* logp_ref,
+                        const float* weight, const float* adv_stats, long long n, double clip_eps_low, double clip_eps_high,
+                        double kl_coef, float* dlogp, float* loss4, void* workspace, size_t workspace_bytes, void* stream);
+/* Loss over P pairs of compared segments (paired log ratios; offsets as pfpn_gae's: segment s = rows [offsets[s],
+ * offsets[s+1]) of the T log-probs, DEVICE int64 [2P+1], ascending, clamped to [0, T]; pair p prefers segment 2p to 2p+1):
+ *   S_s = sum_t w_t (logp_t - logp_ref_t), delta = S_2p - S_2p+1, margin = beta delta,
+ *   kind 0: -(1 - e) log sigma(margin) - e log sigma(-margin) (e = label_smoothing); kind 1: (delta - 1 / (2 beta))^2; mean over P.
+ * logp_ref, weight optional; a step of weight 0 is skipped whatever it holds.  dlogp [T] is written for every row (0 outside all
+ * segments), margin [P], loss3 = {loss, share of pairs with margin > 0, mean margin}.  P <= 2^22. */
+size_t pfpn_preference_workspace_bytes(int P, long long T);
+int pfpn_preference_loss(const float* logp, const float* logp_ref, const float* weight, const int64_t* offsets, int P,
+                         long long T, double beta, double label_smoothing, int kind, float* dlogp, float* margin,
+                         float* loss3, void* workspace, size_t workspace_bytes, void* stream);
+/* Balance loss over the categories of each choice, with counts (keeps particles from dying out, as pfpn_active_stats measures
+ * them: reference a2c.py:346-365).  Over the V rows that mask (uint8 [R], optional) leaves: counts[a,n] = rows whose topk largest
+ * logits hold n (equal ones: lowest index first; -inf never), f = counts / (topk V), mean_prob = mean softmax,
+ *   loss = coef N / A sum_{a,n} f mean_prob (>= coef, = coef when balanced), dlogits (+)= coef N / (A V) p_n (f_n - sum_m f_m p_m).
+ * Masked rows are not read, their gradient is 0 (accumulate: left alone).  N <= 1024, A <= 4096, topk <= min(N, 64). */
+size_t pfpn_balance_workspace_bytes(int R, int A, int N);
+int pfpn_balance_loss(const void* logits, int dtype, long long row_stride, const uint8_t* mask, int R, int A, int N, int topk,
+                      double coef, int accumulate, float* loss, int32_t* counts, float* mean_prob, void* dlogits,
+                      long long grad_stride, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- host utility ------------------------------------------------------------------------- */
 /* CRC-32C (Castagnoli) of a HOST buffer, chained through `crc` (0 for the first call): the per-tensor and
  * per-block checksum of TensorFlow's tensor_bundle checkpoint files, which the reference writes through

@@ -1,0 +1,156 @@
+// Shared device pieces of the policy-objective kernels (categorical log-probs, clipped loss with a KL term, balance loss):
+// logit types, unaligned wide loads, reductions over groups of lanes, the loss head of one row.
+#pragma once
+#include "pfpn_common.h"
+
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+namespace pfpn {
+
+// dtype codes of the C ABI
+enum { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };
+
+struct bf16_t { uint16_t u; };
+struct f16_t { uint16_t u; };
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(bf16_t v) { return __uint_as_float((uint32_t)v.u << 16); }
+__device__ __forceinline__ float to_f32(f16_t v) { return (float)__builtin_bit_cast(_Float16, v.u); }
+// one rounding, to nearest even: the only one between a gradient's 32-bit value and its 16-bit tensor
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ bf16_t from_f32<bf16_t>(float v) {
+    return bf16_t{__builtin_bit_cast(uint16_t, (__bf16)v)};
+}
+template <> __device__ __forceinline__ f16_t from_f32<f16_t>(float v) {
+    return f16_t{__builtin_bit_cast(uint16_t, (_Float16)v)};
+}
+
+// V elements loaded / stored at once from an address that is only element-aligned (rows of an odd length start anywhere;
+// gfx950 global accesses take any alignment, and hipcc emits the wide form for a packed struct)
+template <typename T, int V>
+struct __attribute__((packed, aligned(alignof(T)))) Pack { T v[V]; };
+
+template <typename T, int V>
+__device__ __forceinline__ void load_pack(const T* p, T (&out)[V]) {
+    const Pack<T, V> t = *reinterpret_cast<const Pack<T, V>*>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = t.v[i];
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_pack(T* p, const T (&in)[V]) {
+    Pack<T, V> t;
+#pragma unroll
+    for (int i = 0; i < V; ++i) t.v[i] = in[i];
+    *reinterpret_cast<Pack<T, V>*>(p) = t;
+}
+
+// Reductions over aligned groups of G lanes (2 .. 64), every lane gets the result, no LDS round trip: quad_perm xor 1, xor 2,
+// row_half_mirror (quads of a half row), row_mirror (half rows), then gfx950's row / half-wave swaps.
+template <int CTRL>
+__device__ __forceinline__ uint32_t lane_move(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+template <int G, typename F>
+__device__ __forceinline__ uint32_t group_reduce(uint32_t v, F op) {
+    if (G > 1) v = op(v, lane_move<0xB1>(v));
+    if (G > 2) v = op(v, lane_move<0x4E>(v));
+    if (G > 4) v = op(v, lane_move<0x141>(v));
+    if (G > 8) v = op(v, lane_move<0x140>(v));
+    if (G > 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = op(r[0], r[1]);
+    }
+    if (G > 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = op(r[0], r[1]);
+    }
+    return v;
+}
+template <int G>
+__device__ __forceinline__ float group_max(float v) {
+    return __uint_as_float(group_reduce<G>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }));
+}
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+    return __uint_as_float(group_reduce<G>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+    }));
+}
+template <int G>
+__device__ __forceinline__ uint32_t group_min(uint32_t v) {
+    return group_reduce<G>(v, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+}
+
+// exp(x - m): the difference first (exact where it matters: near the maximum), then ONE v_exp_f32
+__device__ __forceinline__ float exp_below(float x, float m) {
+    return __builtin_amdgcn_exp2f((x - m) * PFPN_LOG2E);
+}
+
+// {max, sum exp(x - max)} of two parts of one axis joined; (-inf, 0) is the empty part
+__device__ __forceinline__ void join_softmax(float& m, float& s, float m2, float s2) {
+    const float mm = fmaxf(m, m2);
+    const float a = (m == mm) ? s : s * exp_below(m, mm);       // (m == mm also where both are -inf or +inf)
+    const float b = (m2 == mm) ? s2 : s2 * exp_below(m2, mm);
+    m = mm;
+    s = a + b;
+}
+
+// ---- the loss head of one row ---------------------------------------------------------------------------------------
+// a = clip((adv - mean) * rstd), r = exp(logp - logp_old), d = logp_ref - logp,
+// loss_row = w (-min(r a, clip(r) a) + c (exp(d) - 1 - d)),   d loss / d logp = w ([not clipped] (-a r) - c (exp(d) - 1)).
+// All in 64 bits: a joint log-prob of many dimensions is some hundreds, its difference to the old one some hundredths, and
+// exp(d) - 1 - d of near log-probs is d^2 / 2 (a row costs two exponentials whatever its width).
+struct HeadArgs {
+    const float* logp_old;
+    const float* adv;
+    const float* logp_ref;      // optional
+    const float* weight;        // optional: 1 / B each
+    const float* stats;         // optional: {mean, rstd, clip_lo, clip_hi}
+    double clip_lo, clip_hi;    // bounds of the ratio
+    double kl_coef;
+    double inv_B;
+};
+struct HeadTerms {
+    double policy, kl, clipped;
+};
+
+__device__ __forceinline__ double policy_head(double logp, size_t b, double w, const HeadArgs& h, HeadTerms& t) {
+    float a = h.adv[b];
+    if (h.stats) a = clip_adv((a - h.stats[0]) * h.stats[1], h.stats[2], h.stats[3]);
+    const double r = exp(logp - (double)h.logp_old[b]);
+    const double held_r = r < h.clip_lo ? h.clip_lo : (r > h.clip_hi ? h.clip_hi : r);
+    const double sur = r * (double)a, held = held_r * (double)a;
+    const bool clipped = held < sur;
+    double g = clipped ? 0.0 : -sur;
+    double kl = 0.0;
+    if (h.logp_ref) {
+        const double d = (double)h.logp_ref[b] - logp;
+        const double em1 = expm1(d);
+        kl = em1 - d;
+        g -= h.kl_coef * em1;
+    }
+    t.policy += w * (clipped ? -held : -sur);
+    t.kl += w * kl;
+    t.clipped += clipped ? w : 0.0;
+    return w * g;
+}
+
+// per-block sums {policy, kl, clipped} -> part[3]; `red` needs 3 * 16 doubles of LDS.  Fixed order.
+__device__ __forceinline__ void block_terms(const HeadTerms& t, double* red, double* part) {
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, nw = (blockDim.x + 63) >> 6;
+    const double a = wave_sum(t.policy), b = wave_sum(t.kl), c = wave_sum(t.clipped);
+    __syncthreads();
+    if (lane == 0) { red[wid * 3] = a; red[wid * 3 + 1] = b; red[wid * 3 + 2] = c; }
+    __syncthreads();
+    if (threadIdx.x < 3) {
+        double s = 0.0;
+        for (int i = 0; i < nw; ++i) s += red[i * 3 + threadIdx.x];
+        part[threadIdx.x] = s;
+    }
+}
+
+}  // namespace pfpn

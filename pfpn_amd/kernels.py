@@ -4,6 +4,7 @@ PyTorch is plumbing here: device memory + the current HIP stream.  Every functio
 shapes/dtypes on the host before launching (a faulting kernel can take the whole node down) and
 launches on torch's current stream, so calls can be captured in a torch.cuda.CUDAGraph.
 """
+import contextlib
 import ctypes
 import os
 
@@ -523,6 +524,261 @@ def resample(loc, logstd, bias, weight, max_active, sum_active, u_resample, u_no
                                  A, N, float(threshold), int(tanh_mode), int(topk), float(fixed_sigma or 0.0), dead.data_ptr(), src.data_ptr(),
                                  _stream()), "pfpn_resample")
     return dead, src
+
+
+# --------------------------------------------------------------------------------------- #
+# policy objectives                                                                        #
+# --------------------------------------------------------------------------------------- #
+_LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_HERE = contextlib.nullcontext()
+
+
+def _on(device):
+    """the device of the tensors, where it is not the current one already"""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _rows(t, n, device, name):
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.float32 and t.is_contiguous()):
+        raise ValueError("%s must be a contiguous float32 CUDA tensor" % name)
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError("%s has shape %s, expected (%d,)" % (name, tuple(t.shape), n))
+    if t.device != device:
+        raise ValueError("%s is on %s, the other tensors on %s" % (name, t.device, device))
+    return t.data_ptr()
+
+
+def _logit_rows(t, name="logits"):
+    """-> (pointer, dtype code, row stride, B, A, N) of categorical logits [B, A, N] or [B, N]; rows may be padded."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _LOGIT_TYPES):
+        raise ValueError("%s must be a float32, bfloat16 or float16 CUDA tensor" % name)
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 3:
+        B, A, N = shape
+        dense = (stride[2] == 1 or N == 1) and (stride[1] == N or A == 1)
+    elif len(shape) == 2:
+        (B, N), A = shape, 1
+        dense = stride[1] == 1 or N == 1
+    else:
+        raise ValueError("%s has shape %s, expected [B, A, N] or [B, N]" % (name, tuple(shape)))
+    if A < 1 or N < 1:
+        raise ValueError("%s has shape %s: no category to choose" % (name, tuple(shape)))
+    ld = stride[0] if B > 1 else A * N
+    if not dense or ld < A * N:
+        raise ValueError("%s: only the rows may be strided (shape %s, strides %s)" % (name, tuple(shape), stride))
+    if A > 4096 or N > 1 << 30:
+        raise ValueError("%s has shape %s: at most 4096 choices of 2^30 categories" % (name, tuple(shape)))
+    return t.data_ptr(), _LOGIT_TYPES[t.dtype], ld, B, A, N
+
+
+def _index(t, logits, name="index"):
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in (torch.int32, torch.int64) and t.is_contiguous()):
+        raise ValueError("%s must be a contiguous int32 or int64 CUDA tensor" % name)
+    if t.shape != logits.shape[:-1] or t.device != logits.device:
+        raise ValueError("%s has shape %s on %s, expected %s on %s" % (name, tuple(t.shape), t.device,
+                                                                       tuple(logits.shape[:-1]), logits.device))
+    return t.data_ptr(), int(t.dtype == torch.int64)
+
+
+def _logit_grad(dlogits, logits):
+    """-> (tensor, pointer, row stride) of the gradient of `logits`; None: a new dense one"""
+    if dlogits is None:
+        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        return dlogits, dlogits.data_ptr(), logits.shape[-1] * (logits.shape[1] if logits.dim() == 3 else 1)
+    ptr, _, ld, B, A, N = _logit_rows(dlogits, "dlogits")
+    if dlogits.shape != logits.shape or dlogits.dtype != logits.dtype or dlogits.device != logits.device:
+        raise ValueError("dlogits is %s %s on %s, expected %s %s on %s" % (
+            tuple(dlogits.shape), dlogits.dtype, dlogits.device, tuple(logits.shape), logits.dtype, logits.device))
+    size = logits.element_size()
+    own, of = ((B - 1) * ld + A * N) * size, ((B - 1) * logits.stride(0) + A * N) * size
+    if B and ptr < logits.data_ptr() + of and logits.data_ptr() < ptr + own:
+        raise ValueError("dlogits overlaps logits")
+    return dlogits, ptr, ld
+
+
+def _clip_bounds(clip_eps):
+    lo, hi = clip_eps if hasattr(clip_eps, "__len__") else (clip_eps, clip_eps)
+    lo, hi = float(lo), float(hi)
+    if not (0.0 <= lo <= 1.0 and hi >= 0.0):
+        raise ValueError("clip_eps is a width e or a pair (low, high), 0 <= low <= 1, high >= 0; got %s" % (clip_eps,))
+    return lo, hi
+
+
+def _scratch(nbytes, device):
+    # a fresh block of torch's allocator per call: ordered with the call's stream, and inside a capture the graph's own
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def categorical_logprob_fwd(logits, index, out=None):
+    """log-prob of the chosen categories: logits [B,A,N] (or [B,N]) float32 / bfloat16 / float16, rows may be padded; index
+    [B,A] ([B]) int32 / int64, outside [0,N): that choice does not count -> logp [B] float32."""
+    pl, dt, ld, B, A, N = _logit_rows(logits)
+    pi, i64 = _index(index, logits)
+    dev = logits.device
+    logp = torch.empty(B, dtype=torch.float32, device=dev) if out is None else out
+    po = _rows(logp, B, dev, "logp")
+    if B == 0:
+        return logp
+    lib = _lib.load()
+    with _on(dev):
+        ws = _scratch(lib.pfpn_categorical_workspace_bytes(B, A, N) if N > 1024 else 0, dev)
+        _lib.check(lib.pfpn_categorical_logprob_fwd(pl, dt, ld, pi, i64, B, A, N, po, ws.data_ptr() if ws is not None else None,
+                                                    ws.numel() if ws is not None else 0, _stream()),
+                   "pfpn_categorical_logprob_fwd")
+    return logp
+
+
+def categorical_logprob_bwd(logits, index, dlogp, dlogits=None):
+    """gradient of sum_b dlogp[b] * logp[b] in the logits' type; `dlogits` given: added to it (as entropy_bwd does)."""
+    pl, dt, ld, B, A, N = _logit_rows(logits)
+    pi, i64 = _index(index, logits)
+    dev = logits.device
+    pg = _rows(dlogp, B, dev, "dlogp")
+    acc = dlogits is not None
+    dlogits, pd, ldd = _logit_grad(dlogits, logits)
+    if B == 0:
+        return dlogits
+    lib = _lib.load()
+    with _on(dev):
+        ws = _scratch(lib.pfpn_categorical_workspace_bytes(B, A, N) if N > 1024 else 0, dev)
+        _lib.check(lib.pfpn_categorical_logprob_bwd(pl, dt, ld, pi, i64, pg, B, A, N, int(acc), pd, ldd,
+                                                    ws.data_ptr() if ws is not None else None,
+                                                    ws.numel() if ws is not None else 0, _stream()),
+                   "pfpn_categorical_logprob_bwd")
+    return dlogits
+
+
+def _head_args(n, dev, logp_old, adv, logp_ref, weight, stats, kl_coef):
+    if kl_coef and logp_ref is None:
+        raise ValueError("kl_coef = %s needs logp_ref" % (kl_coef,))
+    return (_rows(logp_old, n, dev, "logp_old"), _rows(adv, n, dev, "adv"),
+            _rows(logp_ref, n, dev, "logp_ref") if logp_ref is not None else None,
+            _rows(weight, n, dev, "weight") if weight is not None else None,
+            _rows(stats, 4, dev, "adv_stats") if stats is not None else None)
+
+
+def categorical_ppo_fwd_bwd(logits, index, logp_old, adv, logp_ref=None, weight=None, stats=None, clip_eps=0.2, kl_coef=0.0,
+                            out=None):
+    """Clipped policy loss with a KL term on categorical log-probs, forward and backward from the logits in one pass.
+    `clip_eps`: e or (low, high); `logp_ref` [B]: log-probs of the same choices under a reference policy (the KL term's sample,
+    exp(d) - 1 - d with d = logp_ref - logp); `weight` [B]: each row's share of the loss (None: 1/B), 0 skips a row whatever it
+    holds; `stats`: new_adv_stats() / adv_stats().  Returns dict(logp [B], dlogits, loss4 = {loss, policy, kl, clipped share});
+    `out`: such a dict to write into."""
+    pl, dt, ld, B, A, N = _logit_rows(logits)
+    pi, i64 = _index(index, logits)
+    dev = logits.device
+    lo, hi = _clip_bounds(clip_eps)
+    head = _head_args(B, dev, logp_old, adv, logp_ref, weight, stats, kl_coef)
+    if out is None:
+        out = {"logp": torch.empty(B, dtype=torch.float32, device=dev), "dlogits": None,
+               "loss4": torch.empty(4, dtype=torch.float32, device=dev)}
+    else:
+        out = dict(out)
+    out["dlogits"], pd, ldd = _logit_grad(out["dlogits"], logits)
+    po, p4 = _rows(out["logp"], B, dev, "logp"), _rows(out["loss4"], 4, dev, "loss4")
+    if B == 0:
+        out["loss4"].zero_()
+        return out
+    lib = _lib.load()
+    with _on(dev):
+        ws = _scratch(lib.pfpn_categorical_workspace_bytes(B, A, N), dev)
+        _lib.check(lib.pfpn_categorical_ppo_fwd_bwd(pl, dt, ld, pi, i64, *head, B, A, N, lo, hi, float(kl_coef), po, pd, ldd, p4,
+                                                    ws.data_ptr(), ws.numel(), _stream()), "pfpn_categorical_ppo_fwd_bwd")
+    return out
+
+
+def policy_kl_loss(logp, logp_old, adv, logp_ref=None, weight=None, stats=None, clip_eps=0.2, kl_coef=0.0, dlogp=None,
+                   loss4=None):
+    """The loss of categorical_ppo_fwd_bwd on log-probs [n] from elsewhere (logprob_fwd; logprob_bwd carries the result on).
+    -> dlogp [n], loss4; both may be given to write into."""
+    if not isinstance(logp, torch.Tensor) or logp.dim() != 1:
+        raise ValueError("logp must be a [n] tensor")
+    n, dev = logp.shape[0], logp.device
+    pl = _rows(logp, n, dev, "logp")
+    lo, hi = _clip_bounds(clip_eps)
+    head = _head_args(n, dev, logp_old, adv, logp_ref, weight, stats, kl_coef)
+    dlogp = torch.empty(n, dtype=torch.float32, device=dev) if dlogp is None else dlogp
+    loss4 = torch.empty(4, dtype=torch.float32, device=dev) if loss4 is None else loss4
+    pd, p4 = _rows(dlogp, n, dev, "dlogp"), _rows(loss4, 4, dev, "loss4")
+    if n == 0:
+        loss4.zero_()
+        return dlogp, loss4
+    lib = _lib.load()
+    with _on(dev):
+        ws = _scratch(lib.pfpn_policy_kl_workspace_bytes(n), dev)
+        _lib.check(lib.pfpn_policy_kl_loss(pl, *head, n, lo, hi, float(kl_coef), pd, p4, ws.data_ptr(), ws.numel(), _stream()),
+                   "pfpn_policy_kl_loss")
+    return dlogp, loss4
+
+
+_PREFERENCE_KINDS = {"logistic": 0, "squared": 1}
+
+
+def preference_loss(logp, offsets, logp_ref=None, weight=None, beta=0.1, label_smoothing=0.0, kind="logistic"):
+    """Loss over pairs of compared segments of per-step log-probs [T].  offsets [2P+1] int64 (device, ascending): segment s =
+    rows offsets[s] .. offsets[s+1] - 1, pair p prefers segment 2p to segment 2p + 1.  `logp_ref` [T]: the same steps under a
+    reference policy; `weight` [T]: discounts or a mask, 0 skips a step whatever it holds.  kind "logistic" (label_smoothing
+    in [0, 0.5]) or "squared".  -> dlogp [T] (0 outside all segments), margin [P], loss3 = {loss, share won, mean margin}."""
+    if not isinstance(logp, torch.Tensor) or logp.dim() != 1:
+        raise ValueError("logp must be a [T] tensor")
+    T, dev = logp.shape[0], logp.device
+    pl = _rows(logp, T, dev, "logp")
+    if not (isinstance(offsets, torch.Tensor) and offsets.is_cuda and offsets.dtype == torch.int64 and offsets.is_contiguous() and
+            offsets.dim() == 1 and offsets.device == dev):
+        raise ValueError("offsets must be a contiguous int64 [2P + 1] tensor on the log-probs' device")
+    if offsets.shape[0] < 3 or offsets.shape[0] % 2 == 0:
+        raise ValueError("offsets holds %d bounds: an odd number, two segments for each pair, is needed" % offsets.shape[0])
+    P = offsets.shape[0] // 2
+    if P > 1 << 22:
+        raise ValueError("at most 2^22 pairs")
+    if kind not in _PREFERENCE_KINDS:
+        raise ValueError("kind is one of %s" % sorted(_PREFERENCE_KINDS))
+    if not float(beta) > 0.0 or not 0.0 <= float(label_smoothing) <= 0.5:
+        raise ValueError("beta > 0 and label_smoothing in [0, 0.5] are needed")
+    if label_smoothing and kind != "logistic":
+        raise ValueError("label_smoothing belongs to the logistic loss")
+    pr = _rows(logp_ref, T, dev, "logp_ref") if logp_ref is not None else None
+    pw = _rows(weight, T, dev, "weight") if weight is not None else None
+    dlogp = torch.empty(T, dtype=torch.float32, device=dev)
+    margin = torch.empty(P, dtype=torch.float32, device=dev)
+    loss3 = torch.empty(3, dtype=torch.float32, device=dev)
+    lib = _lib.load()
+    with _on(dev):
+        ws = _scratch(lib.pfpn_preference_workspace_bytes(P, T), dev)
+        _lib.check(lib.pfpn_preference_loss(pl, pr, pw, offsets.data_ptr(), P, T, float(beta), float(label_smoothing),
+                                            _PREFERENCE_KINDS[kind], dlogp.data_ptr(), margin.data_ptr(), loss3.data_ptr(),
+                                            ws.data_ptr(), ws.numel(), _stream()), "pfpn_preference_loss")
+    return dlogp, margin, loss3
+
+
+def balance_loss(logits, topk=1, coef=1.0, mask=None, dlogits=None):
+    """Balance loss over the N categories of each choice: logits [R,A,N] (or [R,N]); a row counts for its `topk` largest
+    logits (equal ones: the lowest index first; -inf never); mask [R] bool: rows that count.  `dlogits` given: the gradient
+    is added to it.  -> loss [1] (= coef when balanced), counts [A,N] int32, mean_prob [A,N], dlogits."""
+    pl, dt, ld, R, A, N = _logit_rows(logits)
+    dev, topk = logits.device, int(topk)
+    if N > 1024 or not 1 <= topk <= min(N, 64):
+        raise ValueError("balance_loss: N = %d, topk = %d: N <= 1024 and 1 <= topk <= min(N, 64)" % (N, topk))
+    pm = None
+    if mask is not None:
+        if not (isinstance(mask, torch.Tensor) and mask.is_cuda and mask.dtype in (torch.bool, torch.uint8) and
+                mask.is_contiguous() and mask.shape == (R,) and mask.device == dev):
+            raise ValueError("mask must be a contiguous bool [%d] tensor on %s" % (R, dev))
+        pm = mask.data_ptr()
+    acc = dlogits is not None
+    dlogits, pd, ldd = _logit_grad(dlogits, logits)
+    loss = torch.empty(1, dtype=torch.float32, device=dev)
+    counts = torch.empty(A, N, dtype=torch.int32, device=dev)
+    mean_prob = torch.empty(A, N, dtype=torch.float32, device=dev)
+    if R == 0:
+        return loss.zero_(), counts.zero_(), mean_prob.zero_(), dlogits
+    lib = _lib.load()
+    with _on(dev):
+        ws = _scratch(lib.pfpn_balance_workspace_bytes(R, A, N), dev)
+        _lib.check(lib.pfpn_balance_loss(pl, dt, ld, pm, R, A, N, topk, float(coef), int(acc), loss.data_ptr(), counts.data_ptr(),
+                                         mean_prob.data_ptr(), pd, ldd, ws.data_ptr(), ws.numel(), _stream()),
+                   "pfpn_balance_loss")
+    return loss, counts, mean_prob, dlogits
 
 
 # --------------------------------------------------------------------------------------- #
