@@ -27,6 +27,9 @@ template <> __device__ __forceinline__ f16_t from_f32<f16_t>(float v) {
     return f16_t{__builtin_bit_cast(uint16_t, (_Float16)v)};
 }
 
+template <typename T> struct Bits { typedef uint16_t type; };
+template <> struct Bits<float> { typedef uint32_t type; };
+
 // V elements loaded / stored at once from an address that is only element-aligned (rows of an odd length start anywhere;
 // gfx950 global accesses take any alignment, and hipcc emits the wide form for a packed struct)
 template <typename T, int V>
@@ -45,6 +48,48 @@ __device__ __forceinline__ void store_pack(T* p, const T (&in)[V]) {
     for (int i = 0; i < V; ++i) t.v[i] = in[i];
     *reinterpret_cast<Pack<T, V>*>(p) = t;
 }
+// ... past the caches (gradients larger than the infinity cache: nobody finds them there)
+template <typename T, int V>
+__device__ __forceinline__ void store_pack(T* p, const T (&in)[V], bool stream) {
+    if (stream && (V * sizeof(T)) % 16 == 0) {
+        typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
+        Pack<T, V> t;
+#pragma unroll
+        for (int i = 0; i < V; ++i) t.v[i] = in[i];
+        const Words* w = reinterpret_cast<const Words*>(&t);
+#pragma unroll
+        for (int i = 0; i < (int)(V * sizeof(T) / 16); ++i) __builtin_nontemporal_store(w[i], reinterpret_cast<Words*>(p) + i);
+    } else {
+        store_pack<T, V>(p, in);
+    }
+}
+
+// Wide loads kept in registers as they came, for several passes: `forget` makes the compiler convert them anew in the next
+// pass (it would keep the 32-bit values of 16-bit logits alive, twice the registers).
+template <typename T, int V>
+struct Held {
+    static constexpr int W = V * sizeof(T) / 4;
+    uint32_t w[W];
+    __device__ __forceinline__ void load(const T* p) {
+        struct __attribute__((packed, aligned(alignof(T)))) Words { uint32_t w[W]; };
+        const Words t = *reinterpret_cast<const Words*>(p);
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = t.w[i];
+    }
+    __device__ __forceinline__ void fill(uint32_t v) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = v;
+    }
+    __device__ __forceinline__ void forget() {
+#pragma unroll
+        for (int i = 0; i < W; ++i) asm("" : "+v"(w[i]));
+    }
+    __device__ __forceinline__ float operator[](int i) const {
+        if (sizeof(T) == 4) return __uint_as_float(w[i]);
+        const uint32_t h = (i & 1) ? w[i / 2] >> 16 : w[i / 2] & 0xffffu;
+        return to_f32(__builtin_bit_cast(T, (typename Bits<T>::type)h));
+    }
+};
 
 // Reductions over aligned groups of G lanes (2 .. 64), every lane gets the result, no LDS round trip: quad_perm xor 1, xor 2,
 // row_half_mirror (quads of a half row), row_mirror (half rows), then gfx950's row / half-wave swaps.
@@ -89,6 +134,11 @@ __device__ __forceinline__ uint32_t group_min(uint32_t v) {
 __device__ __forceinline__ float exp_below(float x, float m) {
     return __builtin_amdgcn_exp2f((x - m) * PFPN_LOG2E);
 }
+// the same with log2(e) in two parts (float32's own is off by 1.3e-8, always to the same side: 128 choices add that up)
+__device__ __forceinline__ float exp_below_exact(float x, float m) {
+    const float d = x - m;
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(d, PFPN_LOG2E, d * 1.92596299e-8f));
+}
 
 // {max, sum exp(x - max)} of two parts of one axis joined; (-inf, 0) is the empty part
 __device__ __forceinline__ void join_softmax(float& m, float& s, float m2, float s2) {
@@ -98,6 +148,33 @@ __device__ __forceinline__ void join_softmax(float& m, float& s, float m2, float
     m = mm;
     s = a + b;
 }
+
+// ---- a short axis (N <= 1024) over a group of G lanes: U packs of V consecutive categories a lane -------------------------------
+// Pack u of lane j is the segment's pack u G + j: a pack is one wide access from any alignment, the lanes' packs lie side by side.
+// The segment's last pack is moved down to end at N, so that every access is whole and inside the segment (V <= N): its first
+// categories then belong to the pack before, `own` says which count.
+template <typename T, int G, int E>
+struct Axis {
+    static constexpr int V = E * sizeof(T) <= 24 ? E : 16 / (int)sizeof(T), U = E / V;
+    static_assert(U * V == E, "whole packs");
+    int j, N;
+    __device__ __forceinline__ Axis(int j_, int N_) : j(j_), N(N_) {}
+    __device__ __forceinline__ int lo(int u) const { return (u * G + j) * V; }
+    __device__ __forceinline__ bool has(int u) const { return lo(u) < N; }
+    __device__ __forceinline__ int start(int u) const { return lo(u) < N - V ? lo(u) : N - V; }
+    __device__ __forceinline__ int at(int e) const { return start(e / V) + e % V; }                     // category of element e
+    __device__ __forceinline__ bool own(int e) const { return has(e / V) && at(e) >= lo(e / V); }
+    // (packs past the axis read its last one again: no branch, so that all loads of a thread are in flight together)
+    __device__ __forceinline__ void load(const T* segment, T (&raw)[E]) const {
+#pragma unroll
+        for (int u = 0; u < U; ++u) load_pack<T, V>(segment + start(u), reinterpret_cast<T (&)[V]>(raw[u * V]));
+    }
+    __device__ __forceinline__ void store(T* segment, const T (&o)[E], bool stream) const {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (has(u)) store_pack<T, V>(segment + start(u), reinterpret_cast<const T (&)[V]>(o[u * V]), stream);
+    }
+};
 
 // ---- the loss head of one row ---------------------------------------------------------------------------------------
 // a = clip((adv - mean) * rstd), r = exp(logp - logp_old), d = logp_ref - logp,
@@ -114,29 +191,42 @@ struct HeadArgs {
     double kl_coef;
     double inv_B;
 };
+struct HeadRow {
+    float logp_old, a, logp_ref;
+    double w;
+};
 struct HeadTerms {
     double policy, kl, clipped;
 };
 
-__device__ __forceinline__ double policy_head(double logp, size_t b, double w, const HeadArgs& h, HeadTerms& t) {
-    float a = h.adv[b];
-    if (h.stats) a = clip_adv((a - h.stats[0]) * h.stats[1], h.stats[2], h.stats[3]);
-    const double r = exp(logp - (double)h.logp_old[b]);
+__device__ __forceinline__ HeadRow head_row(const HeadArgs& h, size_t b) {
+    HeadRow r;
+    r.logp_old = h.logp_old[b];
+    r.a = h.adv[b];
+    r.logp_ref = h.logp_ref ? h.logp_ref[b] : 0.f;
+    r.w = h.weight ? (double)h.weight[b] : h.inv_B;
+    if (h.stats) r.a = clip_adv((r.a - h.stats[0]) * h.stats[1], h.stats[2], h.stats[3]);
+    return r;
+}
+
+// -> d loss / d logp of a row of weight != 0; its terms
+__device__ __forceinline__ double policy_head(double logp, const HeadRow& row, const HeadArgs& h, HeadTerms& t) {
+    const double r = exp(logp - (double)row.logp_old);
     const double held_r = r < h.clip_lo ? h.clip_lo : (r > h.clip_hi ? h.clip_hi : r);
-    const double sur = r * (double)a, held = held_r * (double)a;
+    const double sur = r * (double)row.a, held = held_r * (double)row.a;
     const bool clipped = held < sur;
     double g = clipped ? 0.0 : -sur;
     double kl = 0.0;
     if (h.logp_ref) {
-        const double d = (double)h.logp_ref[b] - logp;
+        const double d = (double)row.logp_ref - logp;
         const double em1 = expm1(d);
         kl = em1 - d;
         g -= h.kl_coef * em1;
     }
-    t.policy += w * (clipped ? -held : -sur);
-    t.kl += w * kl;
-    t.clipped += clipped ? w : 0.0;
-    return w * g;
+    t.policy = row.w * (clipped ? -held : -sur);
+    t.kl = row.w * kl;
+    t.clipped = clipped ? row.w : 0.0;
+    return row.w * g;
 }
 
 // per-block sums {policy, kl, clipped} -> part[3]; `red` needs 3 * 16 doubles of LDS.  Fixed order.
