@@ -140,41 +140,198 @@ struct BalArgs {
     const unsigned char* mask;      // optional [R]
     int R, A, N, K;
     double scale;                   // coef N / A
-    int accumulate;
+    int accumulate, stream;
     float* loss;
     int* counts;
     float* mean_prob;
     void* dlogits;
     long long ldd;
-    int AT, RR, tiles, chunks;      // choices and rows side by side in a block; blocks = tiles * chunks
+    int AT, RR, tiles;              // choices and rows side by side in a block
+    int chunks, grad_chunks;        // of rows; blocks = tiles * chunks
     float* slab_p;                  // [chunks][A N]
     uint32_t* slab_n;               // [chunks][A N]
     uint32_t* slab_v;               // [chunks] valid rows
     float* f;                       // [A N] coef N / (A V) f
     double* terms;                  // [blocks of k_bal_reduce]
 };
-constexpr int BAL_NT = 512;
+constexpr int BAL_NT = 576, BAL_COLS = 32;
 
-template <typename T, int G, int E>
-__device__ __forceinline__ void load_segment(const BalArgs& p, bool on, size_t b, int a, int j, float (&x)[E]) {
-    const T* l = static_cast<const T*>(p.logits) + b * p.ld + (size_t)a * p.N;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int n = j + G * e;
-        x[e] = (on && n < p.N) ? to_f32(l[n]) : -INFINITY;
+// Where a group works: its choice, and its row beside the block's other rows
+template <int G>
+struct BalPlace {
+    int tile, chunk, j, al, rr, a;
+    bool mine;
+    long long r0, r1;
+    __device__ __forceinline__ BalPlace(const BalArgs& p, int chunks) {
+        tile = blockIdx.x % p.tiles;
+        chunk = blockIdx.x / p.tiles;
+        j = threadIdx.x % G;
+        const int gid = threadIdx.x / G;
+        al = gid % p.AT;
+        rr = gid / p.AT;
+        a = tile * p.AT + al;
+        mine = rr < p.RR && a < p.A;
+        const long long per = ((long long)p.R + chunks - 1) / chunks;
+        r0 = chunk * per;
+        r1 = r0 + per < p.R ? r0 + per : p.R;
     }
+};
+
+// A group's segment, row after row; past the chunk's end it stays where it is
+template <typename T>
+struct RowWalk {
+    const T* at;
+    long long row;
+    __device__ __forceinline__ RowWalk(const BalArgs& p, long long r0, long long r1, int rr, size_t off) {
+        row = r0 + rr < r1 ? r0 + rr : (r1 > 0 ? r1 - 1 : 0);
+        at = static_cast<const T*>(p.logits) + row * p.ld + off;
+    }
+    __device__ __forceinline__ bool counts(const BalArgs& p) const { return !p.mask || p.mask[row]; }
+    __device__ __forceinline__ void step(const BalArgs& p, long long r1) {
+        const bool on = row + p.RR < r1;
+        row += on ? p.RR : 0;
+        at += on ? p.RR * p.ld : 0;
+    }
+};
+
+// The K-th largest of a group's values, K > 1: every lane sorts its E values once; then up to K rounds of the group's largest head,
+// which all lanes that hold it pop (a group that has popped K is done).  Keys are the float bits ordered as integers.
+__device__ __forceinline__ int order_key(float x) {
+    const int b = __float_as_int(x);            // (-0 below +0: the K-th VALUE is the same either way)
+    return b ^ ((b >> 31) & 0x7fffffff);
+}
+template <int G>
+__device__ __forceinline__ int group_max_key(int v) {
+    return (int)group_reduce<G>((uint32_t)v, [](uint32_t a, uint32_t b) { return (uint32_t)((int)a > (int)b ? (int)a : (int)b); });
+}
+template <int G>
+__device__ __forceinline__ uint32_t group_add(uint32_t v) {
+    return group_reduce<G>(v, [](uint32_t a, uint32_t b) { return a + b; });
+}
+template <int G, int E>
+__device__ __forceinline__ int kth_largest(const int (&keys)[E], int K) {
+    int s[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) s[e] = keys[e];
+    // odd-even transposition, descending
+#pragma unroll
+    for (int r = 0; r < E; ++r)
+#pragma unroll
+        for (int e = r & 1; e + 1 < E; e += 2) {
+            const int hi = s[e] > s[e + 1] ? s[e] : s[e + 1], lo = s[e] > s[e + 1] ? s[e + 1] : s[e];
+            s[e] = hi;
+            s[e + 1] = lo;
+        }
+    const int lane = threadIdx.x & 63;
+    const unsigned long long group = (G == 64 ? ~0ull : ((1ull << (G & 63)) - 1)) << (lane / G * G & 63);
+    int left = K, kth = s[0];
+    for (int k = 0; k < K; ++k) {
+        const int top = group_max_key<G>(s[0]);
+        const unsigned long long held = __builtin_amdgcn_ballot_w64(s[0] == top) & group;
+        if (left > 0) kth = top;
+        const int pop = left > 0 && s[0] == top ? -1 : 0;       // (a mask: hipcc makes an indexed load of a selection)
+        left -= (int)__popcll(held);
+#pragma unroll
+        for (int e = 0; e < E; ++e) s[e] ^= (s[e] ^ (e + 1 < E ? s[e + 1] : (int)0x80000000)) & pop;
+        if (__builtin_amdgcn_ballot_w64(left > 0) == 0) break;
+    }
+    return kth;
 }
 
-template <typename T, int G, int E>
+// ... and for K <= 8, three times cheaper than the rounds (8 of 128: 160 instructions for 16 lanes' lists): every lane's eight
+// largest in order, then the lists of two lanes, of two pairs, ... joined: the eight largest of both are max(a[i], b[7 - i]), a bitonic
+// sequence, which three stages of exchanges put in order.
+__device__ __forceinline__ void exchange(int& a, int& b) {
+    const int hi = a > b ? a : b, lo = a > b ? b : a;
+    a = hi;
+    b = lo;
+}
+__device__ __forceinline__ void bitonic8(int (&s)[8]) {
+#pragma unroll
+    for (int d = 4; d; d >>= 1)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (!(i & d)) exchange(s[i], s[i + d]);
+}
+__device__ __forceinline__ void sort8(int (&s)[8]) {          // odd-even merge sort, descending
+#pragma unroll
+    for (int p = 1; p < 8; p <<= 1)
+#pragma unroll
+        for (int k = p; k; k >>= 1)
+#pragma unroll
+            for (int j = k % p; j + k < 8; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; ++i)
+                    if (i + j + k < 8 && (i + j) / (2 * p) == (i + j + k) / (2 * p)) exchange(s[i + j], s[i + j + k]);
+}
+__device__ __forceinline__ void join8(int (&s)[8], const int (&o)[8]) {
+    int t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = s[i] > o[7 - i] ? s[i] : o[7 - i];
+    bitonic8(t);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = t[i];
+}
+template <int CTRL>
+__device__ __forceinline__ void join8_lanes(int (&s)[8]) {
+    int o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = (int)lane_move<CTRL>((uint32_t)s[i]);
+    join8(s, o);
+}
+template <int G, int E>
+__device__ __forceinline__ int kth_of_eight(const int (&keys)[E], int K) {
+    int s[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = i < E ? keys[i < E ? i : 0] : (int)0x80000000;
+    sort8(s);
+    if (E > 8) {
+        int t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = 8 + i < E ? keys[8 + i < E ? 8 + i : 0] : (int)0x80000000;
+        sort8(t);
+        join8(s, t);
+    }
+    static_assert(E <= 16, "two lists of eight");
+    if (G > 1) join8_lanes<0xB1>(s);
+    if (G > 2) join8_lanes<0x4E>(s);
+    if (G > 4) join8_lanes<0x141>(s);
+    if (G > 8) join8_lanes<0x140>(s);
+    if (G > 16) {
+        int a[8], b[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const auto r = __builtin_amdgcn_permlane16_swap((uint32_t)s[i], (uint32_t)s[i], false, false);
+            a[i] = (int)r[0];
+            b[i] = (int)r[1];
+        }
+        join8(a, b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] = a[i];
+    }
+    if (G > 32) {
+        int a[8], b[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const auto r = __builtin_amdgcn_permlane32_swap((uint32_t)s[i], (uint32_t)s[i], false, false);
+            a[i] = (int)r[0];
+            b[i] = (int)r[1];
+        }
+        join8(a, b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] = a[i];
+    }
+    int kth = s[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) kth = K == i + 1 ? s[i] : kth;
+    return kth;
+}
+
+template <typename T, int G, int E, bool FULL>
 __global__ __launch_bounds__(BAL_NT) void k_bal_stats(BalArgs p) {
     extern __shared__ char lds_raw[];
-    const int tile = blockIdx.x % p.tiles, chunk = blockIdx.x / p.tiles;
-    const int j = threadIdx.x % G, gid = threadIdx.x / G;
-    const int a0 = tile * p.AT, al = gid % p.AT, rr = gid / p.AT, a = a0 + al;
-    const bool mine = rr < p.RR && a < p.A;
-    const int per = (p.R + p.chunks - 1) / p.chunks;
-    const long long r0 = (long long)chunk * per;
-    const long long r1 = r0 + per < p.R ? r0 + per : p.R;
+    const BalPlace<G> at(p, p.chunks);
+    const Axis<T, G, E> ln(at.j, p.N);
     float* sums = reinterpret_cast<float*>(lds_raw);                            // [RR][AT N]
     uint32_t* cnts = reinterpret_cast<uint32_t*>(sums + (size_t)p.RR * p.AT * p.N);    // [AT N]
     for (int i = threadIdx.x; i < p.AT * p.N; i += blockDim.x) cnts[i] = 0;
@@ -183,15 +340,27 @@ __global__ __launch_bounds__(BAL_NT) void k_bal_stats(BalArgs p) {
 #pragma unroll
     for (int e = 0; e < E; ++e) { acc[e] = 0.f; cnt[e] = 0; }
     uint32_t valid = 0;
-    for (long long rb = r0; rb < r1; rb += p.RR) {
-        const long long b = rb + rr;
-        const bool row = mine && b < r1 && (!p.mask || p.mask[b]);
-        float x[E];
-        load_segment<T, G, E>(p, row, (size_t)b, a, j, x);
-        valid += row;
-        float m = -INFINITY;
+    RowWalk<T> walk(p, at.r0, at.r1, at.rr, (size_t)(at.a < p.A ? at.a : p.A - 1) * p.N);
+    T next[E];
+    bool next_on = false;
+    if (at.r0 < at.r1) {
+        ln.load(walk.at, next);
+        next_on = walk.counts(p);
+    }
+    for (long long rb = at.r0; rb < at.r1; rb += p.RR) {
+        const bool row = at.mine && rb + at.rr < at.r1 && next_on;
+        float x[E], m = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < E; ++e) m = fmaxf(m, x[e]);
+        for (int e = 0; e < E; ++e) {
+            x[e] = row && (FULL || ln.own(e)) ? to_f32(next[e]) : -INFINITY;
+            m = fmaxf(m, x[e]);
+        }
+        if (rb + p.RR < at.r1) {                // the next row is on its way meanwhile
+            walk.step(p, at.r1);
+            ln.load(walk.at, next);
+            next_on = walk.counts(p);
+        }
+        valid += row;
         m = group_max<G>(m);
         const float ms = m == -INFINITY ? 0.f : m;
         float ex[E], s = 0.f;
@@ -200,64 +369,114 @@ __global__ __launch_bounds__(BAL_NT) void k_bal_stats(BalArgs p) {
         s = group_sum<G>(s);
         const float inv = s == 0.f ? 0.f : 1.f / s;
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += ex[e] * inv;
-        for (int k = 0; k < p.K; ++k) {
-            if (k) {
-                m = -INFINITY;
+        for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(ex[e], inv, acc[e]);
+        // the chosen: at or above the K-th largest (a closed choice never), of equal ones the first
+        if constexpr (sizeof(T) == 2) {
+            // 16-bit logits leave 13 bits of their 32-bit form free: with the index there no two keys are equal (equal logits are
+            // common at 8 bits of mantissa: ranking them afterwards took as long as all the rest)
+            int keys[E];
 #pragma unroll
-                for (int e = 0; e < E; ++e) m = fmaxf(m, x[e]);
-                m = group_max<G>(m);
+            for (int e = 0; e < E; ++e) {
+                const int b = __float_as_int(x[e] + 0.f);           // (-0 -> +0: equal values)
+                keys[e] = (b ^ ((b >> 31) & 0x7fffe000)) + (0x1fff - ln.at(e));
             }
-            uint32_t at = 0xffffffffu;
+            int kth;
+            if (p.K == 1) {
+                kth = keys[0];
 #pragma unroll
-            for (int e = E - 1; e >= 0; --e)
-                if (x[e] == m) at = j + G * e;
-            at = group_min<G>(at);
-            if (m > -INFINITY) {
+                for (int e = 1; e < E; ++e) kth = keys[e] > kth ? keys[e] : kth;
+                kth = group_max_key<G>(kth);
+            } else {
+                kth = p.K <= 8 ? kth_of_eight<G, E>(keys, p.K) : kth_largest<G, E>(keys, p.K);
+            }
+            constexpr int open = (int)0x80800000;                   // above every key of -inf, below those of finite logits
+            kth = kth > open ? kth : open;
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (at == (uint32_t)(j + G * e)) { cnt[e] += 1; x[e] = -INFINITY; }
+            for (int e = 0; e < E; ++e) cnt[e] += keys[e] >= kth;
+            continue;
+        }
+        float kth = m;
+        if (p.K > 1) {
+            int keys[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) keys[e] = order_key(x[e]);
+            const int key = p.K <= 8 ? kth_of_eight<G, E>(keys, p.K) : kth_largest<G, E>(keys, p.K);
+            kth = __int_as_float(key ^ ((key >> 31) & 0x7fffffff));
+        }
+        // (counted over the wave by the scalar unit: with K open choices or more in every row, more than K a row means equal ones)
+        int taken = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) taken += __popcll(__builtin_amdgcn_ballot_w64(x[e] >= kth && row));
+        const unsigned long long few = __builtin_amdgcn_ballot_w64(row && kth == -INFINITY);
+        if (kth == -INFINITY) kth = -3.402823466e38f;
+        if (few == 0 && taken * G <= p.K * __popcll(__builtin_amdgcn_ballot_w64(row))) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) cnt[e] += x[e] >= kth;
+        } else {
+            // more equal values than room: rank them by index, pack by pack (a pack row is in lane order)
+            uint32_t above = 0, before = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) above += x[e] > kth;
+            const int room = p.K - (int)group_add<G>(above);
+#pragma unroll
+            for (int u = 0; u < ln.U; ++u) {
+                uint32_t mine = 0;
+#pragma unroll
+                for (int v = 0; v < ln.V; ++v) mine += x[u * ln.V + v] == kth;
+                uint32_t lower = mine;                          // inclusive prefix over the group's lanes
+                for (int o = 1; o < G; o <<= 1) {
+                    const uint32_t t = (uint32_t)__shfl_up((int)lower, o, G);
+                    if (at.j >= o) lower += t;
+                }
+                uint32_t rank = before + lower - mine;
+#pragma unroll
+                for (int v = 0; v < ln.V; ++v) {
+                    const int e = u * ln.V + v;
+                    const bool eq = x[e] == kth;
+                    cnt[e] += x[e] > kth || (eq && (int)rank < room);
+                    rank += eq;
+                }
+                before += (uint32_t)__shfl((int)lower, G - 1, G);
             }
         }
     }
     __syncthreads();
-    if (mine) {
+    if (at.mine) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int n = j + G * e;
-            if (n < p.N) {
-                sums[((size_t)rr * p.AT + al) * p.N + n] = acc[e];
-                if (cnt[e]) atomicAdd(&cnts[al * p.N + n], cnt[e]);
+            if (ln.own(e)) {
+                sums[((size_t)at.rr * p.AT + at.al) * p.N + ln.at(e)] = acc[e];
+                if (cnt[e]) atomicAdd(&cnts[at.al * p.N + ln.at(e)], cnt[e]);
             }
         }
     }
     __syncthreads();
     const size_t AN = (size_t)p.A * p.N;
-    const int cols = (p.A - a0 < p.AT ? p.A - a0 : p.AT) * p.N;
+    const int a0 = at.tile * p.AT, cols = (p.A - a0 < p.AT ? p.A - a0 : p.AT) * p.N;
     for (int i = threadIdx.x; i < cols; i += blockDim.x) {
         float s = 0.f;
         for (int q = 0; q < p.RR; ++q) s += sums[(size_t)q * p.AT * p.N + i];
-        p.slab_p[(size_t)chunk * AN + (size_t)a0 * p.N + i] = s;
-        p.slab_n[(size_t)chunk * AN + (size_t)a0 * p.N + i] = cnts[i];
+        p.slab_p[(size_t)at.chunk * AN + (size_t)a0 * p.N + i] = s;
+        p.slab_n[(size_t)at.chunk * AN + (size_t)a0 * p.N + i] = cnts[i];
     }
-    if (tile == 0) {
+    if (at.tile == 0) {
         __syncthreads();
         if (threadIdx.x == 0) cnts[0] = 0;
         __syncthreads();
-        if (al == 0 && j == 0 && valid) atomicAdd(&cnts[0], valid);
+        if (at.al == 0 && at.j == 0 && valid) atomicAdd(&cnts[0], valid);
         __syncthreads();
-        if (threadIdx.x == 0) p.slab_v[chunk] = cnts[0];
+        if (threadIdx.x == 0) p.slab_v[at.chunk] = cnts[0];
     }
 }
 
-// 64 columns x 16 lanes over the slabs
+// 32 columns x 32 lanes over the slabs, eight of them in flight a lane
 __global__ __launch_bounds__(1024) void k_bal_reduce(BalArgs p) {
-    __shared__ double rs[16][64];
-    __shared__ uint32_t rn[16][64];
+    __shared__ double rs[32][BAL_COLS + 1];
+    __shared__ uint32_t rn[32][BAL_COLS + 1];
     __shared__ uint32_t v_all;
     const size_t AN = (size_t)p.A * p.N;
-    const int cl = threadIdx.x & 63, kl = threadIdx.x >> 6;
-    const size_t col = (size_t)blockIdx.x * 64 + cl;
+    const int cl = threadIdx.x % BAL_COLS, kl = threadIdx.x / BAL_COLS;
+    const size_t col = (size_t)blockIdx.x * BAL_COLS + cl;
     if (threadIdx.x == 0) v_all = 0;
     __syncthreads();
     uint32_t v = 0;
@@ -265,79 +484,103 @@ __global__ __launch_bounds__(1024) void k_bal_reduce(BalArgs p) {
     if (v) atomicAdd(&v_all, v);
     double s = 0.0;
     uint32_t n = 0;
-    if (col < AN)
-        for (int k = kl; k < p.chunks; k += 16) {
-            s += (double)p.slab_p[(size_t)k * AN + col];
-            n += p.slab_n[(size_t)k * AN + col];
+    if (col < AN) {
+        for (int k0 = kl; k0 < p.chunks; k0 += 32 * 8) {
+            float fp[8];
+            uint32_t fn[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int k = k0 + 32 * i < p.chunks ? k0 + 32 * i : kl;
+                fp[i] = p.slab_p[(size_t)k * AN + col];
+                fn[i] = p.slab_n[(size_t)k * AN + col];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (k0 + 32 * i < p.chunks) { s += (double)fp[i]; n += fn[i]; }
         }
+    }
     rs[kl][cl] = s;
     rn[kl][cl] = n;
     __syncthreads();
-    if (kl == 0) {
-        for (int i = 1; i < 16; ++i) { s += rs[i][cl]; n += rn[i][cl]; }
-        const double inv_v = v_all ? 1.0 / (double)v_all : 0.0;
-        const double mean = s * inv_v, share = (double)n * inv_v / p.K;
+    if (threadIdx.x < 64) {
         double term = 0.0;
-        if (col < AN) {
-            p.mean_prob[col] = (float)mean;
-            p.counts[col] = (int)n;
-            p.f[col] = (float)(p.scale * inv_v * share);
-            term = share * mean;
+        if (threadIdx.x < BAL_COLS) {
+            s = 0.0;
+            n = 0;
+            for (int i = 0; i < 32; ++i) { s += rs[i][cl]; n += rn[i][cl]; }
+            const double inv_v = v_all ? 1.0 / (double)v_all : 0.0;
+            const double mean = s * inv_v, share = (double)n * inv_v / p.K;
+            if (col < AN) {
+                p.mean_prob[col] = (float)mean;
+                p.counts[col] = (int)n;
+                p.f[col] = (float)(p.scale * inv_v * share);
+                term = share * mean;
+            }
         }
         term = wave_sum(term);
-        if (cl == 0) p.terms[blockIdx.x] = term;
+        if (threadIdx.x == 0) p.terms[blockIdx.x] = term;
     }
 }
 
-template <typename T, int G, int E>
+template <typename T, int G, int E, bool FULL>
 __global__ __launch_bounds__(BAL_NT) void k_bal_grad(BalArgs p) {
-    const int tile = blockIdx.x % p.tiles, chunk = blockIdx.x / p.tiles;
-    const int j = threadIdx.x % G, gid = threadIdx.x / G;
-    const int al = gid % p.AT, rr = gid / p.AT, a = tile * p.AT + al;
-    const bool mine = rr < p.RR && a < p.A;
-    const int per = (p.R + p.chunks - 1) / p.chunks;
-    const long long r0 = (long long)chunk * per;
-    const long long r1 = r0 + per < p.R ? r0 + per : p.R;
+    const BalPlace<G> at(p, p.grad_chunks);
+    const Axis<T, G, E> ln(at.j, p.N);
+    const size_t off = (size_t)(at.a < p.A ? at.a : p.A - 1) * p.N;
+    RowWalk<T> walk(p, at.r0, at.r1, at.rr, off);
     float f[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int n = j + G * e;
-        f[e] = (mine && n < p.N) ? p.f[(size_t)a * p.N + n] : 0.f;
+    for (int e = 0; e < E; ++e) f[e] = p.f[off + ln.at(e)];
+    T next[E];
+    bool next_on = false;
+    if (at.r0 < at.r1) {
+        ln.load(walk.at, next);
+        next_on = walk.counts(p);
     }
-    for (long long rb = r0; rb < r1; rb += p.RR) {
-        const long long b = rb + rr;
-        const bool have = mine && b < r1;
-        const bool row = have && (!p.mask || p.mask[b]);
-        float x[E];
-        load_segment<T, G, E>(p, row, (size_t)b, a, j, x);
-        float m = -INFINITY;
+    for (long long rb = at.r0; rb < at.r1; rb += p.RR) {
+        const long long b = rb + at.rr;
+        const bool have = at.mine && b < at.r1, row = next_on;
+        float x[E], m = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < E; ++e) m = fmaxf(m, x[e]);
+        for (int e = 0; e < E; ++e) {
+            x[e] = to_f32(next[e]);
+            m = fmaxf(m, x[e]);
+        }
+        if (rb + p.RR < at.r1) {                // the next row is on its way meanwhile
+            walk.step(p, at.r1);
+            ln.load(walk.at, next);
+            next_on = walk.counts(p);
+        }
         m = group_max<G>(m);
         if (m == -INFINITY) m = 0.f;
         float s = 0.f, d = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) { x[e] = exp_below(x[e], m); s += x[e]; d += x[e] * f[e]; }
+        for (int e = 0; e < E; ++e) {
+            x[e] = exp_below(x[e], m);
+            const float own = FULL || ln.own(e) ? x[e] : 0.f;
+            s += own;
+            d = __builtin_fmaf(own, f[e], d);
+        }
         s = group_sum<G>(s);
         d = group_sum<G>(d);
-        const float inv = s == 0.f ? 0.f : 1.f / s;
-        d *= inv;
-        if (have) {
-            T* o = static_cast<T*>(p.dlogits) + (size_t)b * p.ldd + (size_t)a * p.N;
+        const float inv = s == 0.f ? 0.f : 1.f / s, di = -d * inv * inv;
+        if (have && (row || !p.accumulate)) {               // (a masked row's gradient: zeros, or left alone)
+            T* to = static_cast<T*>(p.dlogits) + b * p.ldd + off;
+            T o[E];
+            if (p.accumulate) ln.load(to, o);
+            // p_n (f_n - sum f p) with p = x / s, sum f p = d / s
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const int n = j + G * e;
-                if (n < p.N) {
-                    float v = row ? x[e] * inv * (f[e] - d) : 0.f;
-                    if (p.accumulate) v += to_f32(o[n]);
-                    if (row || !p.accumulate) o[n] = from_f32<T>(v);
-                }
+                float v = x[e] * __builtin_fmaf(f[e], inv, di);
+                if (p.accumulate) v += to_f32(o[e]);
+                o[e] = from_f32<T>(row ? v : 0.f);
             }
+            ln.store(to, o, p.stream);
         }
     }
     if (blockIdx.x == 0) {
         __shared__ double red[BAL_NT / 64];
-        const size_t parts = ((size_t)p.A * p.N + 63) / 64;
+        const size_t parts = ((size_t)p.A * p.N + BAL_COLS - 1) / BAL_COLS;
         double t = 0.0;
         for (size_t i = threadIdx.x; i < parts; i += blockDim.x) t += p.terms[i];
         t = wave_sum(t);
@@ -354,47 +597,58 @@ __global__ __launch_bounds__(BAL_NT) void k_bal_grad(BalArgs p) {
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int BAL_MAX_N = 1024, BAL_MAX_K = 64, BAL_MAX_A = 4096;
 
-static int group_width(int N) { return N <= 40 ? 8 : N <= 96 ? 16 : N <= 192 ? 32 : 64; }
+static int group_width(int N) {
+    return N <= 4 ? 4 : N <= 8 ? 2 : N <= 24 ? 4 : N <= 64 ? 8 : N <= 96 ? 16 : N <= 128 ? 8 : N <= 256 ? 32 : 64;
+}
 
 static void bal_shape(BalArgs& p) {
-    const int G = group_width(p.N), groups = BAL_NT / G;
+    const int G = group_width(p.N), groups = BAL_NT / 64 * 64 / G;
     p.AT = p.A < groups ? p.A : groups;
     while (p.AT > 1 && p.AT * p.N > 4096) p.AT = (p.AT + 1) / 2;
     p.RR = groups / p.AT;
     p.tiles = (p.A + p.AT - 1) / p.AT;
-    int c = (1024 + p.tiles - 1) / p.tiles;
-    const int most = (p.R + p.RR - 1) / p.RR;       // a row or more for every group
-    if (c > most) c = most;
-    if (c < 1) c = 1;
-    p.chunks = c;
+    // chunks of rows: two blocks a CU; four rows or more for a group of k_bal_stats (a chunk costs 8 A N bytes of slabs)
+    const long long most = ((long long)p.R + p.RR - 1) / p.RR, fill = (512 + p.tiles - 1) / p.tiles;
+    p.chunks = (int)((most + 3) / 4 < fill ? (most + 3) / 4 : fill);
+    p.grad_chunks = (int)(most < 2 * fill ? most : 2 * fill);
 }
+static size_t bal_terms(const BalArgs& p) { return ((size_t)p.A * p.N + BAL_COLS - 1) / BAL_COLS; }
 static size_t bal_bytes(const BalArgs& p) {
     const size_t AN = (size_t)p.A * p.N;
-    return ((AN + 63) / 64) * sizeof(double) + (size_t)p.chunks * AN * 8 + (size_t)p.chunks * 4 + AN * 4;
+    return bal_terms(p) * sizeof(double) + (size_t)p.chunks * AN * 8 + (size_t)p.chunks * 4 + AN * 4;
 }
 
-template <typename T, int G, int E>
-static void launch_bal(const BalArgs& p, hipStream_t st) {
+template <typename T, int G, int E, bool FULL>
+static void launch_bal_as(const BalArgs& p, hipStream_t st) {
     const int threads = (p.AT * p.RR * G + 63) / 64 * 64;
     const size_t lds = ((size_t)p.RR + 1) * p.AT * p.N * 4;
-    const size_t AN = (size_t)p.A * p.N;
-    hipLaunchKernelGGL((k_bal_stats<T, G, E>), dim3(p.tiles * p.chunks), dim3(threads), lds, st, p);
-    hipLaunchKernelGGL(k_bal_reduce, dim3((unsigned)((AN + 63) / 64)), dim3(1024), 0, st, p);
-    hipLaunchKernelGGL((k_bal_grad<T, G, E>), dim3(p.tiles * p.chunks), dim3(threads), 0, st, p);
+    if (lds > (64u << 10))
+        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&k_bal_stats<T, G, E, FULL>),
+                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    hipLaunchKernelGGL((k_bal_stats<T, G, E, FULL>), dim3(p.tiles * p.chunks), dim3(threads), lds, st, p);
+    hipLaunchKernelGGL(k_bal_reduce, dim3((unsigned)bal_terms(p)), dim3(1024), 0, st, p);
+    hipLaunchKernelGGL((k_bal_grad<T, G, E, FULL>), dim3(p.tiles * p.grad_chunks), dim3(threads), 0, st, p);
+}
+template <typename T, int G, int E>
+static void launch_bal(const BalArgs& p, hipStream_t st) {
+    if (p.N == G * E) launch_bal_as<T, G, E, true>(p, st);      // (no lane without a category: nothing to mask)
+    else launch_bal_as<T, G, E, false>(p, st);
 }
 template <typename T>
 static void pick_bal(const BalArgs& p, hipStream_t st) {
     const int N = p.N;
-    if (N <= 8) launch_bal<T, 8, 1>(p, st);
-    else if (N <= 16) launch_bal<T, 8, 2>(p, st);
-    else if (N <= 24) launch_bal<T, 8, 3>(p, st);
+    if (N <= 4) launch_bal<T, 4, 1>(p, st);
+    else if (N <= 8) launch_bal<T, 2, 4>(p, st);
+    else if (N <= 16) launch_bal<T, 4, 4>(p, st);
+    else if (N <= 24) launch_bal<T, 4, 6>(p, st);
     else if (N <= 32) launch_bal<T, 8, 4>(p, st);
     else if (N <= 40) launch_bal<T, 8, 5>(p, st);
-    else if (N <= 64) launch_bal<T, 16, 4>(p, st);
+    else if (N <= 64) launch_bal<T, 8, 8>(p, st);
     else if (N <= 96) launch_bal<T, 16, 6>(p, st);
-    else if (N <= 128) launch_bal<T, 32, 4>(p, st);
+    else if (N <= 128) launch_bal<T, 8, 16>(p, st);
     else if (N <= 192) launch_bal<T, 32, 6>(p, st);
-    else if (N <= 256) launch_bal<T, 64, 4>(p, st);
+    else if (N <= 256) launch_bal<T, 32, 8>(p, st);
+    else if (N <= 384) launch_bal<T, 64, 6>(p, st);
     else if (N <= 512) launch_bal<T, 64, 8>(p, st);
     else launch_bal<T, 64, 16>(p, st);
 }
@@ -467,11 +721,12 @@ int pfpn_balance_loss(const void* logits, int dtype, long long row_stride, const
     p.scale = coef * (double)N / (double)A;
     p.accumulate = accumulate; p.loss = loss; p.counts = counts; p.mean_prob = mean_prob;
     p.dlogits = dlogits; p.ldd = grad_stride;
+    p.stream = (size_t)R * A * N * (dtype == DT_F32 ? 4 : 2) > (256u << 20);
     bal_shape(p);
     if (!workspace || workspace_bytes < bal_bytes(p)) return PFPN_ERR_WORKSPACE;
     const size_t AN = (size_t)A * N;
     p.terms = static_cast<double*>(workspace);
-    p.slab_p = reinterpret_cast<float*>(p.terms + (AN + 63) / 64);
+    p.slab_p = reinterpret_cast<float*>(p.terms + bal_terms(p));
     p.slab_n = reinterpret_cast<uint32_t*>(p.slab_p + (size_t)p.chunks * AN);
     p.slab_v = p.slab_n + (size_t)p.chunks * AN;
     p.f = reinterpret_cast<float*>(p.slab_v + p.chunks);
