@@ -12,19 +12,54 @@ namespace pfpn {
 // ---------------------------------------------------------------------------------------------------------------------
 // The same loss on log-probs that come from elsewhere (the particle mixture's own density): one pass over [n] vectors.
 // ---------------------------------------------------------------------------------------------------------------------
-__global__ __launch_bounds__(256) void k_policy_rows(const float* __restrict__ logp, HeadArgs h, size_t n,
-                                                     float* __restrict__ dlogp, double* __restrict__ part) {
-    __shared__ double red[3 * 16];
+// Four rows a load, from any alignment.  One block (n <= 4096) finishes the sums itself.
+__device__ __forceinline__ void write_loss4(const double* sums, double kl_coef, float* loss4) {
+    loss4[0] = (float)(sums[0] + kl_coef * sums[1]);
+    loss4[1] = (float)sums[0];
+    loss4[2] = (float)sums[1];
+    loss4[3] = (float)sums[2];
+}
+constexpr long long ROWS_SMALL = 4096;
+
+template <int NT>
+__global__ __launch_bounds__(NT) void k_policy_rows(const float* __restrict__ logp, HeadArgs h, size_t n,
+                                                    float* __restrict__ dlogp, double* __restrict__ part, float* __restrict__ loss4) {
+    __shared__ double red[3 * 16], sums[3];
     HeadTerms t = {0.0, 0.0, 0.0};
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-        const HeadRow row = head_row(h, i);
-        HeadTerms one = {0.0, 0.0, 0.0};
-        dlogp[i] = row.w != 0.0 ? (float)policy_head((double)logp[i], row, h, one) : 0.f;
-        t.policy += one.policy;
-        t.kl += one.kl;
-        t.clipped += one.clipped;
+    float mean = 0.f, rstd = 1.f, lo = -INFINITY, hi = INFINITY;
+    if (h.stats) { mean = h.stats[0]; rstd = h.stats[1]; lo = h.stats[2]; hi = h.stats[3]; }
+    auto one = [&](float lp, float old, float adv, float ref, float w) -> float {
+        const double wd = h.weight ? (double)w : h.inv_B;
+        if (wd == 0.0) return 0.f;
+        const HeadRow row = {old, h.stats ? clip_adv((adv - mean) * rstd, lo, hi) : adv, ref, wd};
+        HeadTerms q;
+        const float g = (float)policy_head((double)lp, row, h, q);
+        t.policy += q.policy;
+        t.kl += q.kl;
+        t.clipped += q.clipped;
+        return g;
+    };
+    const size_t full = n / 4 * 4;
+    for (size_t i = ((size_t)blockIdx.x * NT + threadIdx.x) * 4; i < full; i += (size_t)gridDim.x * NT * 4) {
+        float lp[4], old[4], adv[4], ref[4] = {}, w[4] = {}, d[4];
+        load_pack<float, 4>(logp + i, lp);
+        load_pack<float, 4>(h.logp_old + i, old);
+        load_pack<float, 4>(h.adv + i, adv);
+        if (h.logp_ref) load_pack<float, 4>(h.logp_ref + i, ref);
+        if (h.weight) load_pack<float, 4>(h.weight + i, w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[e] = one(lp[e], old[e], adv[e], ref[e], w[e]);
+        store_pack<float, 4>(dlogp + i, d);
     }
-    block_terms(t, red, part + (size_t)blockIdx.x * 3);
+    const size_t i = full + threadIdx.x;
+    if (blockIdx.x == 0 && i < n)
+        dlogp[i] = one(logp[i], h.logp_old[i], h.adv[i], h.logp_ref ? h.logp_ref[i] : 0.f, h.weight ? h.weight[i] : 0.f);
+    double* out = loss4 ? sums : part + (size_t)blockIdx.x * 3;
+    block_terms(t, red, out);
+    if (loss4) {
+        __syncthreads();
+        if (threadIdx.x == 0) write_loss4(sums, h.kl_coef, loss4);
+    }
 }
 
 // loss4 = {policy + c kl, policy, kl, clipped}: the blocks' sums in a fixed order
@@ -40,12 +75,7 @@ __global__ __launch_bounds__(1024) void k_policy_finish(const double* __restrict
     }
     block_terms(t, red, out);
     __syncthreads();
-    if (threadIdx.x == 0) {
-        loss4[0] = (float)(out[0] + kl_coef * out[1]);
-        loss4[1] = (float)out[0];
-        loss4[2] = (float)out[1];
-        loss4[3] = (float)out[2];
-    }
+    if (threadIdx.x == 0) write_loss4(out, kl_coef, loss4);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -80,7 +110,7 @@ static bool bad_shape(const void* logits, int dtype, long long ld, const void* i
 static bool bad_head(const HeadArgs& h) {
     return !h.logp_old || !h.adv || !(h.clip_lo <= 1.0) || !(h.clip_hi >= 1.0) || (h.kl_coef != 0.0 && !h.logp_ref);
 }
-static int policy_row_blocks(long long n) { return (int)(n / 1024 + 1 < 1024 ? n / 1024 + 1 : 1024); }
+static int policy_row_blocks(long long n) { return (int)(n / 1024 + 1 < 2048 ? n / 1024 + 1 : 2048); }
 
 }  // namespace pfpn
 
@@ -145,11 +175,15 @@ int pfpn_policy_kl_loss(const float* logp, const float* logp_old, const float* a
                         n > 0 ? 1.0 / (double)n : 0.0};
     if (!logp || bad_head(h) || !dlogp || !loss4 || n < 1) return PFPN_ERR_ARG;
     if (!workspace || workspace_bytes < pfpn_policy_kl_workspace_bytes(n)) return PFPN_ERR_WORKSPACE;
-    const int blocks = policy_row_blocks(n);
     double* part = static_cast<double*>(workspace);
-    hipLaunchKernelGGL(k_policy_rows, dim3(blocks), dim3(256), 0, (hipStream_t)stream, logp, h, (size_t)n, dlogp, part);
-    hipLaunchKernelGGL(k_policy_finish, dim3(1), dim3(1024), 0, (hipStream_t)stream, (const double*)part, (size_t)blocks,
-                       kl_coef, loss4);
+    hipStream_t st = (hipStream_t)stream;
+    if (n <= ROWS_SMALL) {
+        hipLaunchKernelGGL((k_policy_rows<1024>), dim3(1), dim3(1024), 0, st, logp, h, (size_t)n, dlogp, part, loss4);
+    } else {
+        const int blocks = policy_row_blocks(n);
+        hipLaunchKernelGGL((k_policy_rows<256>), dim3(blocks), dim3(256), 0, st, logp, h, (size_t)n, dlogp, part, (float*)nullptr);
+        hipLaunchKernelGGL(k_policy_finish, dim3(1), dim3(1024), 0, st, (const double*)part, (size_t)blocks, kl_coef, loss4);
+    }
     PFPN_CHECK_LAUNCH();
     return PFPN_OK;
 }

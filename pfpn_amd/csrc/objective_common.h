@@ -179,8 +179,9 @@ struct Axis {
 // ---- the loss head of one row ---------------------------------------------------------------------------------------
 // a = clip((adv - mean) * rstd), r = exp(logp - logp_old), d = logp_ref - logp,
 // loss_row = w (-min(r a, clip(r) a) + c (exp(d) - 1 - d)),   d loss / d logp = w ([not clipped] (-a r) - c (exp(d) - 1)).
-// All in 64 bits: a joint log-prob of many dimensions is some hundreds, its difference to the old one some hundredths, and
-// exp(d) - 1 - d of near log-probs is d^2 / 2 (a row costs two exponentials whatever its width).
+// The differences of the log-probs are taken in 64 bits (a joint log-prob of many dimensions is some hundreds, its difference to
+// the old one some hundredths), their exponentials in 32: off by 2^-24 (|difference| + 3); exp(d) - 1 - d = d^2 / 2 + ... by its
+// series where it would cancel.  The sums over rows are 64-bit.
 struct HeadArgs {
     const float* logp_old;
     const float* adv;
@@ -209,22 +210,45 @@ __device__ __forceinline__ HeadRow head_row(const HeadArgs& h, size_t b) {
     return r;
 }
 
+// exp(d) - 1 - d; em1 = exp(d) - 1.  |d| < 1: d^2 sum_k d^k / (k + 2)!, the first term left out under 2^-28 of the sum
+__device__ __forceinline__ float kl_sample(float d, float& em1) {
+    if (fabsf(d) < 1.f) {
+        float q = 1.f / 6227020800.f;
+        q = __builtin_fmaf(q, d, 1.f / 479001600.f);
+        q = __builtin_fmaf(q, d, 1.f / 39916800.f);
+        q = __builtin_fmaf(q, d, 1.f / 3628800.f);
+        q = __builtin_fmaf(q, d, 1.f / 362880.f);
+        q = __builtin_fmaf(q, d, 1.f / 40320.f);
+        q = __builtin_fmaf(q, d, 1.f / 5040.f);
+        q = __builtin_fmaf(q, d, 1.f / 720.f);
+        q = __builtin_fmaf(q, d, 1.f / 120.f);
+        q = __builtin_fmaf(q, d, 1.f / 24.f);
+        q = __builtin_fmaf(q, d, 1.f / 6.f);
+        q = __builtin_fmaf(q, d, 0.5f);
+        const float kl = q * d * d;
+        em1 = d + kl;
+        return kl;
+    }
+    em1 = expf(d) - 1.f;
+    return em1 - d;
+}
+
 // -> d loss / d logp of a row of weight != 0; its terms
 __device__ __forceinline__ double policy_head(double logp, const HeadRow& row, const HeadArgs& h, HeadTerms& t) {
-    const double r = exp(logp - (double)row.logp_old);
-    const double held_r = r < h.clip_lo ? h.clip_lo : (r > h.clip_hi ? h.clip_hi : r);
-    const double sur = r * (double)row.a, held = held_r * (double)row.a;
+    const float r = expf((float)(logp - (double)row.logp_old));
+    const float lo = (float)h.clip_lo, hi = (float)h.clip_hi;
+    const float held_r = r < lo ? lo : (r > hi ? hi : r);
+    const float sur = r * row.a, held = held_r * row.a;
     const bool clipped = held < sur;
-    double g = clipped ? 0.0 : -sur;
-    double kl = 0.0;
+    double g = clipped ? 0.0 : -(double)sur;
+    float kl = 0.f;
     if (h.logp_ref) {
-        const double d = (double)row.logp_ref - logp;
-        const double em1 = expm1(d);
-        kl = em1 - d;
-        g -= h.kl_coef * em1;
+        float em1;
+        kl = kl_sample((float)((double)row.logp_ref - logp), em1);
+        g -= h.kl_coef * (double)em1;
     }
-    t.policy = row.w * (clipped ? -held : -sur);
-    t.kl = row.w * kl;
+    t.policy = row.w * (clipped ? -(double)held : -(double)sur);
+    t.kl = row.w * (double)kl;
     t.clipped = clipped ? row.w : 0.0;
     return row.w * g;
 }

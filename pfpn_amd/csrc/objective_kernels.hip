@@ -41,16 +41,52 @@ __device__ __forceinline__ void slice_of(const PrefArgs& p, int s, int part, lon
     lo = a + part * width < b ? a + part * width : b;
     hi = lo + width < b ? lo + width : b;
 }
-// a step of weight 0 is not read any further: what stands there does not matter
-__device__ __forceinline__ double step_gap(const PrefArgs& p, long long t) {
-    const float w = p.weight ? p.weight[t] : 1.f;
-    if (w == 0.f) return 0.0;
-    const double d = (double)p.logp[t] - (p.logp_ref ? (double)p.logp_ref[t] : 0.0);
-    return p.weight ? d * (double)w : d;
+// w (logp - logp_ref) of one step; a step of weight 0: 0, whatever stands there
+__device__ __forceinline__ double step_gap(float lp, float ref, float w) {
+    return w == 0.f ? 0.0 : ((double)lp - (double)ref) * (double)w;
+}
+// a thread's share of rows [lo, hi): four steps a load (from any alignment), `id` of `n` threads
+__device__ __forceinline__ double span_sum(const PrefArgs& p, long long lo, long long hi, int id, int n) {
+    double v = 0.0;
+    const long long full = lo + (hi - lo) / 4 * 4;
+    for (long long t = lo + 4ll * id; t < full; t += 4ll * n) {
+        float a[4], r[4] = {0.f, 0.f, 0.f, 0.f}, w[4] = {1.f, 1.f, 1.f, 1.f};
+        load_pack<float, 4>(p.logp + t, a);
+        if (p.logp_ref) load_pack<float, 4>(p.logp_ref + t, r);
+        if (p.weight) load_pack<float, 4>(p.weight + t, w);
+        v += (step_gap(a[0], r[0], w[0]) + step_gap(a[1], r[1], w[1])) + (step_gap(a[2], r[2], w[2]) + step_gap(a[3], r[3], w[3]));
+    }
+    const long long t = full + id;
+    if (t < hi) v += step_gap(p.logp[t], p.logp_ref ? p.logp_ref[t] : 0.f, p.weight ? p.weight[t] : 1.f);
+    return v;
+}
+// ... and its share of their gradients
+__device__ __forceinline__ float step_grad(double g, float w) { return w == 0.f ? 0.f : (float)(g * (double)w); }
+__device__ __forceinline__ void span_grad(const PrefArgs& p, long long lo, long long hi, int id, int n, double g) {
+    const float gf = (float)g;
+    const long long full = lo + (hi - lo) / 4 * 4;
+    for (long long t = lo + 4ll * id; t < full; t += 4ll * n) {
+        float d[4] = {gf, gf, gf, gf};
+        if (p.weight) {
+            float w[4];
+            load_pack<float, 4>(p.weight + t, w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d[i] = step_grad(g, w[i]);
+        }
+        store_pack<float, 4>(p.dlogp + t, d);
+    }
+    const long long t = full + id;
+    if (t < hi) p.dlogp[t] = p.weight ? step_grad(g, p.weight[t]) : gf;
+}
+// rows outside every segment have no gradient
+__device__ __forceinline__ void outside_zero(const PrefArgs& p, long long id, long long n) {
+    const long long first = p.offsets[0] < 0 ? 0 : p.offsets[0], last = p.offsets[2 * (size_t)p.P];
+    for (long long t = id; t < first && t < p.T; t += n) p.dlogp[t] = 0.f;
+    for (long long t = (last < 0 ? 0 : last) + id; t < p.T; t += n) p.dlogp[t] = 0.f;
 }
 
 // loss of one pair -> d loss / d delta (of the mean); fills terms and margin when `write`
-__device__ __forceinline__ double pair_head(const PrefArgs& p, int pair, double delta, bool write) {
+__device__ __forceinline__ double pair_head(const PrefArgs& p, int pair, double delta, bool write, double* terms) {
     const double m = p.beta * delta;
     double loss, slope;
     if (p.kind == 0) {
@@ -67,49 +103,84 @@ __device__ __forceinline__ double pair_head(const PrefArgs& p, int pair, double 
     }
     if (write) {
         p.margin[pair] = (float)m;
-        p.terms[(size_t)pair * 3] = loss;
-        p.terms[(size_t)pair * 3 + 1] = m > 0 ? 1.0 : 0.0;
-        p.terms[(size_t)pair * 3 + 2] = m;
+        terms[(size_t)pair * 3] = loss;
+        terms[(size_t)pair * 3 + 1] = m > 0 ? 1.0 : 0.0;
+        terms[(size_t)pair * 3 + 2] = m;
     }
     return slope / (double)p.P;
 }
 
+// Few steps: ONE block, a wave per pair in turn (a launch costs more than the work).
+constexpr int PREF_SMALL_P = 128, PREF_SMALL_T = 16384;
+__global__ __launch_bounds__(1024) void k_pref_small(PrefArgs p, float* __restrict__ loss3) {
+    __shared__ double terms[PREF_SMALL_P * 3];
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    for (int pair = wid; pair < p.P; pair += 16) {
+        long long a0, a1, b0, b1;
+        segment_of(p, 2 * pair, a0, a1);
+        segment_of(p, 2 * pair + 1, b0, b1);
+        const double delta = wave_sum(span_sum(p, a0, a1, lane, 64)) - wave_sum(span_sum(p, b0, b1, lane, 64));
+        const double g = pair_head(p, pair, delta, lane == 0, terms);
+        span_grad(p, a0, a1, lane, 64, g);
+        span_grad(p, b0, b1, lane, 64, -g);
+    }
+    outside_zero(p, threadIdx.x, 1024);
+    __syncthreads();
+    if (wid < 3) {
+        double t = 0.0;
+        for (int i = lane; i < p.P; i += 64) t += terms[i * 3 + wid];
+        t = wave_sum(t);
+        if (lane == 0) loss3[wid] = (float)(t / (double)p.P);
+    }
+}
+
+// Many pairs: a block per pair, sums and gradients in one launch.
+__global__ __launch_bounds__(256) void k_pref_pairs(PrefArgs p) {
+    __shared__ double red[8];
+    if (blockIdx.x >= (unsigned)p.P) {
+        outside_zero(p, (long long)(blockIdx.x - p.P) * 256 + threadIdx.x, (long long)(gridDim.x - p.P) * 256);
+        return;
+    }
+    const int pair = blockIdx.x;
+    long long a0, a1, b0, b1;
+    segment_of(p, 2 * pair, a0, a1);
+    segment_of(p, 2 * pair + 1, b0, b1);
+    const double va = wave_sum(span_sum(p, a0, a1, threadIdx.x, 256)), vb = wave_sum(span_sum(p, b0, b1, threadIdx.x, 256));
+    if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6] = va; red[4 + (threadIdx.x >> 6)] = vb; }
+    __syncthreads();
+    const double delta = (((red[0] + red[1]) + red[2]) + red[3]) - (((red[4] + red[5]) + red[6]) + red[7]);
+    const double g = pair_head(p, pair, delta, threadIdx.x == 0, p.terms);
+    span_grad(p, a0, a1, threadIdx.x, 256, g);
+    span_grad(p, b0, b1, threadIdx.x, 256, -g);
+}
+
+// Few, long segments: a block per piece of one; its sum, then (every block joining its pair's pieces, in order) its gradients.
 __global__ __launch_bounds__(256) void k_pref_sums(PrefArgs p) {
     __shared__ double red[4];
     const int s = blockIdx.x / p.splits, part = blockIdx.x % p.splits;
     long long lo, hi;
     slice_of(p, s, part, lo, hi);
-    double v = 0.0;
-    for (long long t = lo + threadIdx.x; t < hi; t += 256) v += step_gap(p, t);
-    v = wave_sum(v);
+    const double v = wave_sum(span_sum(p, lo, hi, threadIdx.x, 256));
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     if (threadIdx.x == 0) p.sums[blockIdx.x] = ((red[0] + red[1]) + red[2]) + red[3];
 }
 
 __global__ __launch_bounds__(256) void k_pref_grad(PrefArgs p) {
-    const long long blocks = 2ll * p.P * p.splits;
+    const unsigned blocks = 2u * p.P * p.splits;
     if (blockIdx.x >= blocks) {
-        // rows outside every segment have no gradient
-        const long long first = p.offsets[0] < 0 ? 0 : p.offsets[0], last = p.offsets[2 * (size_t)p.P];
-        const long long at = (blockIdx.x - blocks) * 256 + threadIdx.x, step = (gridDim.x - blocks) * 256;
-        for (long long t = at; t < first && t < p.T; t += step) p.dlogp[t] = 0.f;
-        for (long long t = (last < 0 ? 0 : last) + at; t < p.T; t += step) p.dlogp[t] = 0.f;
+        outside_zero(p, (long long)(blockIdx.x - blocks) * 256 + threadIdx.x, (long long)(gridDim.x - blocks) * 256);
         return;
     }
     const int s = blockIdx.x / p.splits, part = blockIdx.x % p.splits, pair = s >> 1;
     const double* sums = p.sums + (size_t)pair * 2 * p.splits;
-    double a = 0.0, b = 0.0;
-    for (int i = 0; i < p.splits; ++i) { a += sums[i]; b += sums[p.splits + i]; }
-    double g = pair_head(p, pair, a - b, threadIdx.x == 0 && part == 0 && (s & 1) == 0);
-    if (s & 1) g = -g;
+    const int lane = threadIdx.x & 63;
+    double d = 0.0;
+    for (int i = lane; i < p.splits; i += 64) d += sums[i] - sums[p.splits + i];
+    const double g = pair_head(p, pair, wave_sum(d), threadIdx.x == 0 && part == 0 && (s & 1) == 0, p.terms);
     long long lo, hi;
     slice_of(p, s, part, lo, hi);
-    const float gf = (float)g;
-    for (long long t = lo + threadIdx.x; t < hi; t += 256) {
-        const float w = p.weight ? p.weight[t] : 1.f;
-        p.dlogp[t] = p.weight ? (w == 0.f ? 0.f : (float)(g * (double)w)) : gf;
-    }
+    span_grad(p, lo, hi, threadIdx.x, 256, (s & 1) ? -g : g);
 }
 
 __global__ __launch_bounds__(1024) void k_pref_finish(const double* __restrict__ terms, int P, float* __restrict__ loss3) {
@@ -693,8 +764,17 @@ int pfpn_preference_loss(const float* logp, const float* logp_ref, const float* 
     hipStream_t st = (hipStream_t)stream;
     const unsigned blocks = 2u * (unsigned)P * (unsigned)p.splits;
     const unsigned outside = (unsigned)(T / 4096 + 1 < 64 ? T / 4096 + 1 : 64);
-    hipLaunchKernelGGL(k_pref_sums, dim3(blocks), dim3(256), 0, st, p);
-    hipLaunchKernelGGL(k_pref_grad, dim3(blocks + outside), dim3(256), 0, st, p);
+    if (P <= PREF_SMALL_P && T <= PREF_SMALL_T) {
+        hipLaunchKernelGGL(k_pref_small, dim3(1), dim3(1024), 0, st, p, loss3);
+        PFPN_CHECK_LAUNCH();
+        return PFPN_OK;
+    }
+    if (p.splits == 1) {
+        hipLaunchKernelGGL(k_pref_pairs, dim3((unsigned)P + outside), dim3(256), 0, st, p);
+    } else {
+        hipLaunchKernelGGL(k_pref_sums, dim3(blocks), dim3(256), 0, st, p);
+        hipLaunchKernelGGL(k_pref_grad, dim3(blocks + outside), dim3(256), 0, st, p);
+    }
     hipLaunchKernelGGL(k_pref_finish, dim3(1), dim3(1024), 0, st, (const double*)p.terms, P, loss3);
     PFPN_CHECK_LAUNCH();
     return PFPN_OK;

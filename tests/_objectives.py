@@ -69,7 +69,9 @@ def rounded(value, bound, dtype):
 
 
 def head(logp, old, adv, ref, w, lo, hi, c, stats=None, err=None):
-    """-> dlogp, its bound for log-probs off by `err`, loss4 (64 bits)"""
+    """-> dlogp, its bound for log-probs off by `err`, loss4 (64 bits).  The kernels take the differences of log-probs in 64 bits and
+    round them once, the exponentials in 32: exp is off by |argument| u and a step (2 u), its product with the advantage by u;
+    exp(d) - 1 by (|d| + 2) u exp(d) + u (|d| < 1: by its series, under 8 u of itself)."""
     a = adv.double()
     if stats is not None:
         s = stats.double()
@@ -83,15 +85,17 @@ def head(logp, old, adv, ref, w, lo, hi, c, stats=None, err=None):
     g = torch.where(clipped, torch.zeros_like(sur), -sur)
     kl = torch.zeros_like(r)
     lip = sur.abs()
+    own = sur.abs() * ((logp - old.double()).abs() + 4) * U
     if ref is not None:
         d = ref.double() - logp
         kl = torch.expm1(d) - d
         g = g - c * torch.expm1(d)
         lip = lip + c * torch.exp(d)
+        own = own + c * ((d.abs() + 3) * torch.exp(d) + 8 * torch.expm1(d).abs()) * U
     zero = torch.zeros_like(g)
     sums = [torch.where(live, w * t, zero).sum() for t in (pol + c * kl, pol, kl, clipped.double())]
     dlogp = torch.where(live, w * g, zero)
-    bound = U * dlogp.abs()
+    bound = U * dlogp.abs() + torch.where(live, w.abs() * own, zero)
     if stats is not None:
         bound = bound + 3 * U * torch.where(live, w.abs() * sur.abs() * (1 + adv.double().abs() + stats.double()[0].abs()), zero)
     if err is not None:
