@@ -539,13 +539,14 @@ def _on(device):
 
 
 def _rows(t, n, device, name):
+    if isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.device == device and t.is_cuda and \
+            t.dim() == 1 and t.numel() == n and t.is_contiguous():
+        return t.data_ptr()
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.float32 and t.is_contiguous()):
         raise ValueError("%s must be a contiguous float32 CUDA tensor" % name)
     if t.dim() != 1 or t.shape[0] != n:
         raise ValueError("%s has shape %s, expected (%d,)" % (name, tuple(t.shape), n))
-    if t.device != device:
-        raise ValueError("%s is on %s, the other tensors on %s" % (name, t.device, device))
-    return t.data_ptr()
+    raise ValueError("%s is on %s, the other tensors on %s" % (name, t.device, device))
 
 
 def _logit_rows(t, name="logits"):
@@ -583,7 +584,7 @@ def _index(t, logits, name="index"):
 def _logit_grad(dlogits, logits):
     """-> (tensor, pointer, row stride) of the gradient of `logits`; None: a new dense one"""
     if dlogits is None:
-        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        dlogits = torch.empty_like(logits, memory_format=torch.contiguous_format)
         return dlogits, dlogits.data_ptr(), logits.shape[-1] * (logits.shape[1] if logits.dim() == 3 else 1)
     ptr, _, ld, B, A, N = _logit_rows(dlogits, "dlogits")
     if dlogits.shape != logits.shape or dlogits.dtype != logits.dtype or dlogits.device != logits.device:
@@ -670,14 +671,16 @@ def categorical_ppo_fwd_bwd(logits, index, logp_old, adv, logp_ref=None, weight=
     lo, hi = _clip_bounds(clip_eps)
     head = _head_args(B, dev, logp_old, adv, logp_ref, weight, stats, kl_coef)
     if out is None:
-        out = {"logp": torch.empty(B, dtype=torch.float32, device=dev), "dlogits": None,
-               "loss4": torch.empty(4, dtype=torch.float32, device=dev)}
+        logp, loss4 = torch.empty(B, dtype=torch.float32, device=dev), torch.empty(4, dtype=torch.float32, device=dev)
+        dlogits, pd, ldd = _logit_grad(None, logits)
+        po, p4 = logp.data_ptr(), loss4.data_ptr()
     else:
-        out = dict(out)
-    out["dlogits"], pd, ldd = _logit_grad(out["dlogits"], logits)
-    po, p4 = _rows(out["logp"], B, dev, "logp"), _rows(out["loss4"], 4, dev, "loss4")
+        logp, loss4 = out["logp"], out["loss4"]
+        dlogits, pd, ldd = _logit_grad(out["dlogits"], logits)
+        po, p4 = _rows(logp, B, dev, "logp"), _rows(loss4, 4, dev, "loss4")
+    out = {"logp": logp, "dlogits": dlogits, "loss4": loss4}
     if B == 0:
-        out["loss4"].zero_()
+        loss4.zero_()
         return out
     lib = _lib.load()
     with _on(dev):
@@ -751,10 +754,11 @@ def preference_loss(logp, offsets, logp_ref=None, weight=None, beta=0.1, label_s
     return dlogp, margin, loss3
 
 
-def balance_loss(logits, topk=1, coef=1.0, mask=None, dlogits=None):
+def balance_loss(logits, topk=1, coef=1.0, mask=None, dlogits=None, out=None):
     """Balance loss over the N categories of each choice: logits [R,A,N] (or [R,N]); a row counts for its `topk` largest
     logits (equal ones: the lowest index first; -inf never); mask [R] bool: rows that count.  `dlogits` given: the gradient
-    is added to it.  -> loss [1] (= coef when balanced), counts [A,N] int32, mean_prob [A,N], dlogits."""
+    is added to it.  `out` = (loss, counts, mean_prob): tensors to write into.
+    -> loss [1] (= coef when balanced), counts [A,N] int32, mean_prob [A,N], dlogits."""
     pl, dt, ld, R, A, N = _logit_rows(logits)
     dev, topk = logits.device, int(topk)
     if N > 1024 or not 1 <= topk <= min(N, 64):
@@ -767,9 +771,15 @@ def balance_loss(logits, topk=1, coef=1.0, mask=None, dlogits=None):
         pm = mask.data_ptr()
     acc = dlogits is not None
     dlogits, pd, ldd = _logit_grad(dlogits, logits)
-    loss = torch.empty(1, dtype=torch.float32, device=dev)
-    counts = torch.empty(A, N, dtype=torch.int32, device=dev)
-    mean_prob = torch.empty(A, N, dtype=torch.float32, device=dev)
+    if out is None:
+        loss = torch.empty(1, dtype=torch.float32, device=dev)
+        counts = torch.empty(A, N, dtype=torch.int32, device=dev)
+        mean_prob = torch.empty(A, N, dtype=torch.float32, device=dev)
+    else:
+        loss, counts, mean_prob = out
+        _typed(counts, torch.int32, A, N, name="counts"), _f32(mean_prob, A, N, name="mean_prob"), _rows(loss, 1, dev, "loss")
+        if counts.device != dev or mean_prob.device != dev:
+            raise ValueError("counts and mean_prob belong on %s" % dev)
     if R == 0:
         return loss.zero_(), counts.zero_(), mean_prob.zero_(), dlogits
     lib = _lib.load()

@@ -75,7 +75,7 @@ class A2CNetwork(ActorCriticNetwork):
 class ParticleFilteringA2CNetwork(A2CNetwork):
     def __init__(self, action_lower_bound, action_upper_bound, init_sigma=None, fixed_sigma=False,
                  particles=50, resample=3, resample_interval=2000, resample_threshold=None,
-                 normalize_policy_output=False, **kwargs):
+                 normalize_policy_output=False, balance_beta=None, preference_beta=0.1, preference_smoothing=0.0, **kwargs):
         self.action_lower_bound = None if action_lower_bound is None else np.asarray(action_lower_bound, dtype=np.float64)
         self.action_upper_bound = None if action_upper_bound is None else np.asarray(action_upper_bound, dtype=np.float64)
         super().__init__(**kwargs)
@@ -99,6 +99,15 @@ class ParticleFilteringA2CNetwork(A2CNetwork):
         self.normalize_policy_output = False                      # tanh squash after the mixture (unused)
         self.normalize_policy_output_ = bool(normalize_policy_output)   # tanh squash before the mixture
         self.train_flag = 0
+        # balance_beta: weight of the balance loss over the particles (they die where the weights of a dimension collapse on a few);
+        # preference_beta / _smoothing: train_preference's loss
+        self.balance_beta = balance_beta
+        self.preference_beta, self.preference_smoothing = float(preference_beta), float(preference_smoothing)
+        if balance_beta and self.particles > 1024:
+            raise ValueError("balance_beta: at most 1024 particles")
+        if not self.preference_beta > 0.0 or not 0.0 <= self.preference_smoothing <= 0.5:
+            raise ValueError("preference_beta > 0 and preference_smoothing in [0, 0.5] are needed")
+        self._reference = None
 
     # -- parameters ------------------------------------------------------------------------------
     def build_policy_params(self, store, in_dim):
@@ -138,6 +147,11 @@ class ParticleFilteringA2CNetwork(A2CNetwork):
             self.train_ops.append(self.resample_tick)
         else:
             self.max_active = self.sum_active = None
+        if self.trainable and self.balance_beta:
+            # (loss, counts, mean weights) of the latest learner step, also where it was a replay
+            self.balance_out = (torch.zeros(1, dtype=torch.float32, device=self.device),
+                                torch.zeros(A, N, dtype=torch.int32, device=self.device),
+                                torch.zeros(A, N, dtype=torch.float32, device=self.device))
         if self.normalize_state and self.trainable:
             self.local_update_variables = ["state_normalizer/mean", "state_normalizer/std"] + self.local_update_variables
 
@@ -225,6 +239,87 @@ class ParticleFilteringA2CNetwork(A2CNetwork):
         self.last_entropy = policy.entropy()
         self.last_entropy_mask = mask
         policy.entropy_backward(dH, dlogits)
+
+    def _balance_term(self, policy, dlogits, mask=None):
+        """loss += balance_beta * N / A sum_a sum_n f P over the particles' weights of the (valid) rows: its gradient is added
+        into dlogits; the loss itself joins the loss tensor at the end of the step (`_add_balance`)."""
+        policy.balance(self.balance_beta, mask=None if mask is None else mask != 0, dlogits=dlogits, out=self.balance_out)
+
+    def _add_balance(self, loss):
+        loss[:2].add_(self.balance_out[0])
+
+    # -- a frozen copy of the policy -------------------------------------------------------------------
+    def set_reference(self):
+        """Freeze the policy as it is now (trunk, head, particles) as the reference of the KL term (`kl_coef`) and of
+        train_preference.  Not part of a checkpoint: call it again after restoring one.  Steps captured earlier follow."""
+        if self._reference is None:
+            self._reference = self.store.flat.clone()
+        else:
+            self._reference.copy_(self.store.flat)
+
+    def _reference_log_prob(self, x, action):
+        """log-prob [B] of `action` under the frozen policy on the normalised states x."""
+        ref = self.store.views_of(self._reference)
+        stack = self.trunk if self.trunk is not None else self.actor_trunk
+        ha = stack.forward(x, slot="reference", params=ref)[0]
+        logits = torch.addmm(ref["actor/fc_policy/bias"], ha, ref["actor/fc_policy/weight"])
+        return MixtureGaussianDistribution(logits, ref["actor/samples"], ref["actor/samples_std"],
+                                           self.normalize_policy_output_).log_prob(action)
+
+    def compute_preference_gradients(self, state, action, offsets, weight=None):
+        """Forward + backward of the loss over preferred pairs of trajectory segments (kernels.preference_loss): state [T,S],
+        action [T,A], offsets [2P+1] int64 (segment s = rows offsets[s] .. offsets[s+1]-1, pair p prefers 2p to 2p+1), weight [T]
+        optional (discounts, a mask).  Log ratios are taken to the reference where set_reference() was called.  The critic
+        gets no gradient.  Gradients land in self.store.grad; returns loss3 (device): {loss, share of pairs won, mean margin}."""
+        B = state.shape[0]
+        self._ensure_buffers(B)
+        deferred = self._deferred_jobs(B)
+        x = self.prologue(state, deferred=deferred)
+        logp_ref = self._reference_log_prob(x, action) if self._reference is not None else None
+        st = self.store
+        if deferred is not None:
+            ha, hc = self._trunks_forward(x, value_head=(st["critic/fc3/weight"], st["critic/fc3/bias"], self.value_buf),
+                                          masks=True)
+        else:
+            ha, hc = self._trunks_forward(x)
+        policy = MixtureGaussianDistribution(self._policy_logits(ha), self.loc, self.logstd, self.normalize_policy_output_)
+        dlogp, margin, loss3 = kernels.preference_loss(policy.log_prob(action), offsets, logp_ref, weight,
+                                                       self.preference_beta, self.preference_smoothing)
+        dlogits, dloc, dlogstd = policy.log_prob_backward(action, dlogp)
+        dlogits = dlogits.view(B, -1)
+        st.g("actor/samples").copy_(dloc)
+        st.g("actor/samples_std").copy_(dlogstd)
+        if self.fixed_sigma:
+            st.g("actor/samples_std").zero_()
+        if self.balance_beta:
+            self._balance_term(policy, dlogits)
+            loss3 = loss3.clone()
+            loss3[:1].add_(self.balance_out[0])
+        self._backward_heads(ha, hc, dlogits, torch.zeros(B, dtype=torch.float32, device=self.device), fused_db=False,
+                             deferred=deferred)
+        if deferred is not None:
+            self._finish_deferred(deferred, allow_norm=not self.fixed_sigma)
+        return loss3
+
+    def train_preference(self, sess, optimizer, ops, state, action, offsets, weight=None):
+        """One learner step on compared segments (host arrays or tensors; compute_preference_gradients).
+        Returns ((loss, share of pairs won, mean margin), extra_fetches)."""
+        st = self._to_dev(state).view(-1, self.S)
+        ac = self._to_dev(action).view(-1, self.n_actions)
+        if st.shape[0] == 0 or st.shape[0] != ac.shape[0]:
+            raise ValueError("train_preference: %d states, %d actions" % (st.shape[0], ac.shape[0]))
+        offs = torch.as_tensor(offsets, dtype=torch.int64)
+        if not offs.is_cuda and (int(offs[0]) < 0 or int(offs[-1]) > st.shape[0] or bool((offs[1:] < offs[:-1]).any())):
+            raise ValueError("train_preference: offsets ascend within [0, %d]" % st.shape[0])
+        offs = offs.to(self.device).contiguous()
+        w = None if weight is None else self._to_dev(weight).view(-1)
+        loss3 = self.compute_preference_gradients(st, ac, offs, w)
+        optimizer.apply(self)
+        loss = [float(v) for v in loss3.cpu().numpy()]
+        kernels.check_faults()
+        extra = [self.global_step if o in ("global_step", "step") else (o() if callable(o) else None)
+                 for o in (ops if hasattr(ops, "__len__") else ([ops] if ops else []))]
+        return tuple(loss), extra
 
     def _entropy_value(self):
         H = self.last_entropy.sum(1)
@@ -320,6 +415,9 @@ class ParticleFilteringA2CNetwork(A2CNetwork):
         self.store.g("actor/samples_std").copy_(dlogstd)
         if self.entropy_beta:
             self._entropy_term(policy, dlogits, B, mask, loss4[3] if mask is not None else None)
+        if self.balance_beta:
+            self._balance_term(policy, dlogits, mask)
+            self._add_balance(loss4)
         if self.fixed_sigma:
             self.store.g("actor/samples_std").zero_()
         self._backward_heads(ha, hc, dlogits, dvalue, fused_db=False, deferred=deferred)

@@ -43,6 +43,8 @@ def ddpg_network_wrapper(base_class):
             kwargs.setdefault("normalize_policy_output", True)              # ddpg.py:25-26
             kwargs["fixed_sigma"], kwargs["init_sigma"] = True, act_noise   # ddpg.py:48-50
             super().__init__(**kwargs)
+            if self.balance_beta:
+                raise NotImplementedError("balance_beta belongs to the policy-gradient networks (PPO, A2C, V-trace)")
             self.twin_q, self.policy_delay, self.tau = twin_q, int(policy_delay), tau
             self.act_noise, self.target_noise = float(act_noise), float(target_noise)
             self.reward, self.not_terminal = "reward", "not_terminal"

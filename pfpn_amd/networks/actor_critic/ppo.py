@@ -21,9 +21,14 @@ __all__ = ["ParticleFilteringClipPPONetwork"]
 
 def clip_ppo_network_wrapper(a2c_base_class):
     class ClipPPONetwork(a2c_base_class):
-        def __init__(self, epsilon=0.2, **kwargs):
+        def __init__(self, epsilon=0.2, kl_coef=0.0, **kwargs):
             super().__init__(**kwargs)
             self.epsilon = epsilon
+            self.kl_coef = float(kl_coef or 0.0)       # weight of the KL term to the policy set_reference() froze
+            if not self.kl_coef >= 0.0:
+                raise ValueError("kl_coef >= 0 is needed")
+            if self.kl_coef and self.normalize_policy_output_:
+                raise NotImplementedError("kl_coef with a tanh policy is not built (no PPO setting has one)")
             self.running_log_prob = "pi_running"
             self.running_value = "value_running"
 
@@ -44,11 +49,14 @@ def clip_ppo_network_wrapper(a2c_base_class):
             """Forward + backward of loss = policy_loss + value_loss_coef*value_loss on device tensors.
             Gradients land in self.store.grad; returns loss3 (device): {loss, policy_loss, value_loss*coef}.
             No host synchronisation: capturable in a hipGraph."""
+            if self.kl_coef and self._reference is None:
+                raise RuntimeError("kl_coef needs a reference policy: call set_reference() first")
             B = state.shape[0]
             st = self.store
             self._ensure_buffers(B)
             deferred = self._deferred_jobs(B, fused_mixture=True)
             x = self.prologue(state, advantage, deferred=deferred)   # normalised state, state-norm EMA, advantage moments
+            logp_ref = self._reference_log_prob(x, action) if self.kl_coef else None
             w3, b3 = st["critic/fc3/weight"], st["critic/fc3/bias"]
             if deferred is not None:
                 ha, hc = self._trunks_forward(x, value_head=(w3, b3, self.value_buf), masks=True)
@@ -62,13 +70,17 @@ def clip_ppo_network_wrapper(a2c_base_class):
             # fc_policy bias gradient (column sums of dlogits), saving a 20 MB pass
             # (N > 64: the two-launch composition leaves dloc / dlogstd / dbias / loss3 final, nothing of it is deferred)
             composed = deferred is not None and self._mix_slabs.get("composed", False)
-            fused_db = not self.entropy_beta
+            fused_db = not self.entropy_beta and not self.balance_beta
             gbias = st.g("actor/fc_policy/bias")
-            slabs = deferred is not None and not composed
-            out = kernels.ppo_mixture_fwd_bwd(policy.logits, action, self.loc, self.logstd, log_prob, advantage, v,
-                                              value, self.adv_stats, self.epsilon, self.value_loss_coef,
-                                              out=self.train_out, dbias=gbias if fused_db else None,
-                                              finalize=not slabs, ws=self.ws_mix if slabs else None)
+            slabs = deferred is not None and not composed and logp_ref is None
+            if logp_ref is not None:
+                out = self._kl_composition(policy, action, logp_ref, log_prob, advantage, v, value,
+                                           gbias if fused_db else None)
+            else:
+                out = kernels.ppo_mixture_fwd_bwd(policy.logits, action, self.loc, self.logstd, log_prob, advantage, v,
+                                                  value, self.adv_stats, self.epsilon, self.value_loss_coef,
+                                                  out=self.train_out, dbias=gbias if fused_db else None,
+                                                  finalize=not slabs, ws=self.ws_mix if slabs else None)
             dlogits = out["dlogits"]
             if slabs:
                 # dloc / dlogstd / dbias / loss3 stay as per-block slabs until the step's single reduce launch
@@ -82,12 +94,31 @@ def clip_ppo_network_wrapper(a2c_base_class):
                                                      self.value_loss_coef, out["loss3"]))
             if self.entropy_beta:
                 self._entropy_term(policy, dlogits, B)
+            if self.balance_beta:
+                self._balance_term(policy, dlogits)
             self._backward_heads(ha, hc, dlogits, out["dvalue"], fused_db, deferred=deferred)
             if deferred is not None:
                 self._finish_deferred(deferred, allow_norm=not self.fixed_sigma)
             if self.fixed_sigma:
                 out["dlogstd"].zero_()
+            if self.balance_beta:
+                self._add_balance(out["loss3"])        # (after the launch that finishes the loss)
             return out["loss3"]
+
+        def _kl_composition(self, policy, action, logp_ref, log_prob, advantage, v, value, dbias):
+            """The step's loss with its KL term as launches of its own: log-probs -> clipped loss + KL (kernels.policy_kl_loss)
+            and value loss -> the mixture's backward.  Same outputs as the fused kernel; loss3 = {loss, policy loss with its KL
+            term, value loss * coef}."""
+            out = self.train_out
+            kernels.logprob_fwd(policy.logits, action, self.loc, self.logstd, out=out["logp"])
+            kernels.ppo_loss(out["logp"], log_prob, advantage, v, value, self.adv_stats, self.epsilon, self.value_loss_coef,
+                             dvalue=out["dvalue"], loss3=out["loss3"])
+            dlogp, loss4 = kernels.policy_kl_loss(out["logp"], log_prob, advantage, logp_ref, stats=self.adv_stats,
+                                                  clip_eps=self.epsilon, kl_coef=self.kl_coef)
+            kernels.logprob_bwd(policy.logits, action, self.loc, self.logstd, dlogp, out=out, dbias=dbias)
+            out["loss3"][1:2].copy_(loss4[:1])
+            torch.add(out["loss3"][1:2], out["loss3"][2:3], out=out["loss3"][:1])
+            return out
 
         def stage_next_prologue(self, state, action, value, log_prob, advantage):
             """multi-step captures: hand the NEXT step's prologue to this step's optimiser launch (graphs.py)"""

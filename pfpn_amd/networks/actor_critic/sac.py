@@ -32,6 +32,8 @@ def sac_network_wrapper(base_class):
             if "normalize_policy_output" not in kwargs:
                 kwargs["normalize_policy_output"] = True          # sac.py:15-16
             super().__init__(**kwargs)
+            if self.balance_beta:
+                raise NotImplementedError("balance_beta belongs to the policy-gradient networks (PPO, A2C, V-trace)")
             self.alpha = alpha       # replaced by exp(log_alpha) for the trainable net (sac.py:36-39)
             self.batch_actor = True        # (tests flip these on an instance: the one-pass-per-input reference form)
             self.batch_critic = True

@@ -56,6 +56,27 @@ class MixtureGaussianDistribution(object):
             return torch.atanh(value).contiguous()  # utils.py:124
         return value.contiguous()
 
+    # -- the categorical weights: drawn indices, balance --------------------------------------------
+    def index_log_prob(self, k=None):
+        """joint log-prob [B] of particle indices k [B,A] under the weights (default: those of the last `sample` / `mean`,
+        utils.py:187-194); an index outside [0, N) leaves its dimension out."""
+        return kernels.categorical_logprob_fwd(self.logits.view(-1, self.A, self.N), self.dis_action if k is None else k)
+
+    def index_log_prob_backward(self, dlogp, k=None, dlogits=None):
+        """gradient of sum_b dlogp[b] * index_log_prob[b] w.r.t. the logits, [B,A*N] (added to `dlogits` when given)."""
+        if dlogits is not None:
+            dlogits = dlogits.view(-1, self.A, self.N)
+        return kernels.categorical_logprob_bwd(self.logits.view(-1, self.A, self.N), self.dis_action if k is None else k, dlogp,
+                                               dlogits).view(-1, self.A * self.N)
+
+    def balance(self, coef=1.0, topk=1, mask=None, dlogits=None, out=None):
+        """balance loss of the weights over the batch: -> loss [1], counts [A,N], mean weights [A,N], gradient [B,A*N]
+        (added to `dlogits` when given; kernels.balance_loss)."""
+        if dlogits is not None:
+            dlogits = dlogits.view(-1, self.A, self.N)
+        loss, counts, mean, d = kernels.balance_loss(self.logits.view(-1, self.A, self.N), topk, coef, mask, dlogits, out)
+        return loss, counts, mean, d.view(-1, self.A * self.N)
+
     # -- entropy -------------------------------------------------------------------------------
     def entropy(self):
         """categorical entropy of the weights, [B,A] (utils.py:146-151)."""

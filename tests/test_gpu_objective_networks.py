@@ -1,0 +1,249 @@
+"""GPU: the policy objectives inside the networks' learner steps (KL term to a frozen policy, balance loss, preference steps)
+against 64-bit autograd of the same losses, eager against captured steps, and the distribution's index log-probs."""
+import math
+import os
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+S, A, N = 11, 3, 8
+
+
+def make(dev, cls="ParticleFilteringClipPPONetwork", hidden=(64, 32), critic=None, seed=5, **over):
+    from pfpn_amd import networks
+    opts = dict(common_net_shape=[], actor_net_shape=list(hidden), critic_net_shape=list(critic or hidden), value_loss_coef=0.5,
+                gamma=0.95, normalize_state=True, clip_state=5.0, normalize_advantage=True, particles=N, resample=-1,
+                resample_interval=10 ** 6)
+    opts.update(over)
+    net = getattr(networks, cls)(trainable=True, state_shape=[S], action_shape=[A], action_lower_bound=-np.ones(A),
+                                 action_upper_bound=np.ones(A), device=dev, seed=seed, **opts)
+    net.init()
+    return net
+
+
+def spread_out(net, seed, scale=0.25):
+    """weights as after some training, so that no unit and no particle is degenerate"""
+    g = torch.Generator().manual_seed(seed)
+    for k, v in net.variables().items():
+        if "samples" not in k:
+            v.copy_((torch.randn(v.shape, generator=g) * scale / math.sqrt(max(1, v.shape[0] / 8))).to(v.device))
+
+
+def twin(params, x, action=None):
+    """64-bit forward of actor, critic and mixture from named parameters"""
+    def trunk(p):
+        h = x
+        for i in (1, 2):
+            h = torch.clamp(h @ params["%s/fc%d/weight" % (p, i)] + params["%s/fc%d/bias" % (p, i)].view(-1), 0, 6)
+        return h
+    ha, hc = trunk("actor"), trunk("critic")
+    logits = (ha @ params["actor/fc_policy/weight"] + params["actor/fc_policy/bias"]).view(-1, A, N)
+    v = (hc @ params["critic/fc3/weight"] + params["critic/fc3/bias"]).view(-1)
+    if action is None:
+        return logits, v
+    loc, ls = params["actor/samples"], params["actor/samples_std"]
+    z = (action.unsqueeze(-1) - loc) / ls.exp()
+    dens = -0.5 * z * z - ls - 0.5 * math.log(2 * math.pi)
+    return logits, v, torch.logsumexp(torch.log_softmax(logits, -1) + dens, -1).sum(-1)
+
+
+def doubles(net, grad=True):
+    return {k: v.detach().double().cpu().clone().requires_grad_(grad) for k, v in net.variables().items()}
+
+
+def batch(B, seed):
+    rng = np.random.default_rng(seed)
+    return {"state": rng.normal(0, 1.2, (B, S)).astype(np.float32), "action": rng.uniform(-1, 1, (B, A)).astype(np.float32),
+            "value": rng.normal(0, .1, B).astype(np.float32), "advantage": rng.normal(0, 1, B).astype(np.float32)}
+
+
+def compare(net, params, what):
+    for k, g in net.gradients().items():
+        want = params[k].grad
+        want = torch.zeros_like(params[k]) if want is None else want
+        got = g.detach().double().cpu().view(want.shape)
+        scale = float(want.abs().max())
+        # the bound of the networks' own step tests: 2e-4 of the tensor's largest entry (fp32 GEMMs and sums)
+        assert float((got - want).abs().max()) <= 2e-4 * scale + 1e-9, (what, k)
+
+
+def balance_twin(logits, mask=None):
+    p = torch.softmax(logits, -1)
+    pick = torch.nn.functional.one_hot(logits.detach().argmax(-1), N).double()
+    m = torch.ones(logits.shape[0], dtype=torch.float64) if mask is None else mask
+    f, P = (pick * m.view(-1, 1, 1)).sum(0) / m.sum(), (p * m.view(-1, 1, 1)).sum(0) / m.sum()
+    return N / A * (f * P).sum()
+
+
+@pytest.mark.parametrize("hidden,critic", [((64, 32), None), ((64, 32), (48, 32))])
+@pytest.mark.parametrize("kl,balance", [(0.3, None), (0.0, 0.4), (0.3, 0.4)])
+def test_ppo_step_with_kl_and_balance(dev, hidden, critic, kl, balance):
+    net = make(dev, hidden=hidden, critic=critic, kl_coef=kl, balance_beta=balance)
+    spread_out(net, 1)
+    if kl:
+        with pytest.raises(RuntimeError, match="set_reference"):
+            net.compute_gradients(*[torch.zeros(4, *s, device=dev) for s in ((S,), (A,), (), (), ())])
+    net.set_reference()
+    frozen = doubles(net, False)
+    g = torch.Generator().manual_seed(9)
+    for v in net.variables().values():
+        v.add_(0.02 * torch.randn(v.shape, generator=g).to(dev))
+    B = 64
+    b = batch(B, 3)
+    params = doubles(net)
+    x = torch.clamp(torch.from_numpy(b["state"]).double(), -5, 5)
+    act = torch.from_numpy(b["action"]).double()
+    logits, v, logp = twin(params, x, act)
+    r = np.exp(0.15 * np.random.default_rng(4).normal(size=B))
+    r[np.abs(r - 0.8) < 0.02] = 0.85
+    r[np.abs(r - 1.2) < 0.02] = 1.15
+    old = (logp.detach().numpy() - np.log(r)).astype(np.float32)
+    adv = torch.from_numpy(b["advantage"]).double()
+    na = (adv - adv.mean()) / (adv.std(unbiased=False) + 1e-8)
+    ratio = torch.exp(logp - torch.from_numpy(old).double())
+    pol = -torch.minimum(ratio * na, ratio.clamp(0.8, 1.2) * na).mean()
+    if kl:
+        with torch.no_grad():
+            ref = twin(frozen, x, act)[2]
+        d = ref - logp
+        pol = pol + kl * (torch.expm1(d) - d).mean()
+    if balance:
+        pol = pol + balance * balance_twin(logits)
+    val = 0.5 * ((v - (adv + torch.from_numpy(b["value"]).double())) ** 2).mean()
+    (pol + val).backward()
+    args = [torch.from_numpy(t).to(dev) for t in (b["state"], b["action"], b["value"], old, b["advantage"])]
+    loss3 = net.compute_gradients(*args)
+    compare(net, params, (kl, balance))
+    want = torch.stack([pol + val, pol, val]).detach()
+    want = want.detach()
+    assert float((loss3.double().cpu() - want).abs().max()) < 2e-5 * float(want.abs().max())
+    if balance:
+        pick = logits.detach().argmax(-1)
+        counts = torch.stack([torch.bincount(pick[:, a], minlength=N) for a in range(A)])
+        assert torch.equal(net.balance_out[1].cpu().long(), counts)
+
+
+def test_a2c_step_with_balance(dev):
+    net = make(dev, "ParticleFilteringA2CNetwork", balance_beta=0.4)
+    spread_out(net, 2)
+    B, b = 32, batch(32, 5)
+    params = doubles(net)
+    x = torch.clamp(torch.from_numpy(b["state"]).double(), -5, 5)
+    logits, v, logp = twin(params, x, torch.from_numpy(b["action"]).double())
+    adv, vt = torch.from_numpy(b["advantage"]).double(), torch.from_numpy(b["value"]).double()
+    na = (adv - adv.mean()) / (adv.std(unbiased=False) + 1e-8)
+    loss = -(logp * na).mean() + 0.5 * ((v - vt) ** 2).mean() + 0.4 * balance_twin(logits)
+    loss.backward()
+    dt = {k: torch.from_numpy(t).to(dev) for k, t in b.items()}
+    loss4 = net._pg_gradients(dt["state"], dt["action"], lambda lp, val: (dt["value"], dt["advantage"], None))
+    compare(net, params, "a2c")
+    want = float(loss.detach())
+    assert abs(float(loss4[0]) - want) < 2e-5 * abs(want)
+
+
+@pytest.mark.parametrize("with_reference", [False, True])
+@pytest.mark.parametrize("T", [40, 61])         # (61: the launch-per-piece form of the step)
+def test_preference_step(dev, T, with_reference):
+    net = make(dev, preference_beta=0.7, preference_smoothing=0.05)
+    spread_out(net, 3)
+    frozen = None
+    if with_reference:
+        net.set_reference()
+        frozen = doubles(net, False)
+        g = torch.Generator().manual_seed(2)
+        for v in net.variables().values():
+            v.add_(0.05 * torch.randn(v.shape, generator=g).to(dev))
+    b = batch(T, 8)
+    offs = [0, 7, 15, 15, 33]
+    w = np.random.default_rng(1).uniform(0.5, 1, T).astype(np.float32)
+    w[3] = 0.0
+    params = doubles(net)
+    x = torch.clamp(torch.from_numpy(b["state"]).double(), -5, 5)
+    act = torch.from_numpy(b["action"]).double()
+    logp = twin(params, x, act)[2]
+    gap = logp
+    if with_reference:
+        gap = logp - twin(frozen, x, act)[2]
+    gap = gap * torch.from_numpy(w).double()
+    s = [gap[a:e].sum() for a, e in zip(offs[:-1], offs[1:])]
+    m = 0.7 * torch.stack([s[0] - s[1], s[2] - s[3]])
+    loss = (-0.95 * torch.nn.functional.logsigmoid(m) - 0.05 * torch.nn.functional.logsigmoid(-m)).mean()
+    loss.backward()
+    args = (torch.from_numpy(b["state"]).to(dev), torch.from_numpy(b["action"]).to(dev), torch.tensor(offs, device=dev),
+            torch.from_numpy(w).to(dev))
+    loss3 = net.compute_preference_gradients(*args)
+    # (a log-prob is off by 1e-5 of itself: the ledger of the mixture kernels)
+    want = float(loss.detach())
+    assert abs(float(loss3[0]) - want) < 1e-4 * abs(want)
+    compare(net, params, "preference")
+
+
+def test_train_preference_api(dev):
+    from pfpn_amd.models import SyncReplicasApplier
+    net = make(dev, balance_beta=0.1)
+    opt = SyncReplicasApplier(net, [{"names": None, "lr": 1e-3}], norm_clip=1.0, world_size=1)
+    b = batch(50, 1)
+    before = {k: v.clone() for k, v in net.variables().items()}
+    for _ in range(3):
+        (loss, won, margin), extra = net.train_preference(None, opt, ["global_step"], b["state"], b["action"], [0, 10, 25, 40, 50])
+        assert math.isfinite(loss) and 0.0 <= won <= 1.0 and math.isfinite(margin)
+    assert extra == [net.global_step] and any(not torch.equal(v, before[k]) for k, v in net.variables().items() if "actor" in k)
+    for bad in ([0, 10, 5], [0, 10, 51], [-1, 10, 20], [0, 10]):
+        with pytest.raises(ValueError):
+            net.train_preference(None, opt, [], b["state"], b["action"], bad)
+    with pytest.raises(ValueError):
+        net.train_preference(None, opt, [], b["state"], b["action"][:20], [0, 10, 20])
+
+
+@pytest.mark.parametrize("round_rows", [0, 512])
+def test_captured_steps_equal_eager_ones(dev, monkeypatch, round_rows):
+    """minibatch steps with the KL term and the balance loss: the replayed steps leave the eager steps' bits, the counts of the
+    latest step included, and a reference frozen anew after the capture is the one replays use"""
+    from pfpn_amd.models import SyncReplicasApplier
+    got = []
+    for graphs in ("0", "1"):
+        monkeypatch.setenv("PFPN_GRAPH_TRAIN", graphs)
+        net = make(dev, kl_coef=0.2, balance_beta=0.3)
+        spread_out(net, 4)
+        net.set_reference()
+        opt = SyncReplicasApplier(net, [{"names": None, "lr": 1e-3}], norm_clip=1.0, world_size=1)
+        losses = []
+        if round_rows:
+            b = batch(round_rows, 2)
+            b["log_prob"] = np.random.default_rng(0).normal(-4, .3, round_rows).astype(np.float32)
+            names = ["state", "action", "value", "log_prob", "advantage"]
+            for r in range(4):
+                plan = [np.random.default_rng(r * 10 + i).permutation(round_rows)[:32] for i in range(10)]
+                losses += [l for l, _ in net.train_round(opt, [], names, b, plan)]
+        else:
+            for it in range(12):
+                b = batch(32, it)
+                lp = np.random.default_rng(it).normal(-4, .3, 32).astype(np.float32)
+                losses.append(net.train(None, opt, [], b["state"], b["action"], b["value"], lp, b["advantage"])[0])
+                if it == 8:
+                    net.set_reference()
+        got.append((losses, {k: v.clone() for k, v in net.variables().items()}, [t.clone() for t in net.balance_out]))
+    assert got[0][0] == got[1][0]
+    for k, v in got[0][1].items():
+        assert torch.equal(v, got[1][1][k]), k
+    assert all(torch.equal(a, b) for a, b in zip(got[0][2], got[1][2])) and int(got[0][2][1].sum()) == 32 * A
+
+
+def test_index_log_prob_of_drawn_particles(dev):
+    from pfpn_amd.networks.utils import MixtureGaussianDistribution
+    logits, loc = torch.randn(20, A * N, device=dev), torch.randn(A, N, device=dev)
+    d = MixtureGaussianDistribution(logits, loc, torch.zeros(A, N, device=dev))
+    d.sample()
+    want = torch.log_softmax(logits.double().view(-1, A, N), -1).gather(-1, d.dis_action.long().unsqueeze(-1)).sum((1, 2))
+    assert float((d.index_log_prob().double() - want).abs().max()) < 2e-6
+    up = torch.randn(20, device=dev)
+    x = logits.double().view(-1, A, N).requires_grad_(True)
+    (torch.log_softmax(x, -1).gather(-1, d.dis_action.long().unsqueeze(-1)).sum((1, 2)) * up.double()).sum().backward()
+    assert float((d.index_log_prob_backward(up).double().view(-1, A, N) - x.grad).abs().max()) < 2e-6
+    loss, counts, mean, grad = d.balance(coef=2.0)
+    assert counts.sum() == 20 * A and grad.shape == (20, A * N) and abs(float(mean.sum()) - A) < 1e-5
+    base = torch.ones(20, A * N, device=dev)
+    d.balance(coef=2.0, dlogits=base)
+    assert float((base - 1 - grad).abs().max()) < 2e-7

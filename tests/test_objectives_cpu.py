@@ -93,3 +93,17 @@ def test_balance_entry_point_refuses():
     for change in (dict(ws=None), dict(n=need - 1)):
         assert call(**change) == 3, change
     assert lib.pfpn_balance_workspace_bytes(10, 1, 2000) == 0
+
+
+def test_network_options():
+    from pfpn_amd import networks
+    base = dict(trainable=True, state_shape=[5], action_shape=[2], action_lower_bound=[-1, -1], action_upper_bound=[1, 1],
+                common_net_shape=[], critic_net_shape=[8], actor_net_shape=[8])
+    for bad in (dict(kl_coef=-0.1), dict(preference_beta=0.0), dict(preference_smoothing=0.6), dict(balance_beta=0.1, particles=1025)):
+        with pytest.raises(ValueError):
+            networks.ParticleFilteringClipPPONetwork(**base, **bad)
+    with pytest.raises(NotImplementedError):
+        networks.ParticleFilteringClipPPONetwork(**base, kl_coef=0.1, normalize_policy_output=True)
+    for cls in ("ParticleFilteringSACNetwork", "ParticleFilteringDDPGNetwork"):
+        with pytest.raises(NotImplementedError, match="balance_beta"):
+            getattr(networks, cls)(**base, balance_beta=0.1)
