@@ -41,7 +41,7 @@ int cat_splits(int B, int A, int N);
 // the chosen category, -1 where it is outside the axis (that choice does not enter the row); no branch on the index type
 __device__ __forceinline__ int chosen_in(const CatArgs& p, size_t i) {
     const int* at = static_cast<const int*>(p.index) + (i << p.index64);
-    const int lo = at[0], hi = p.index64 ? at[p.index64] : lo >> 31;
+    const int lo = at[0], second = at[p.index64], hi = p.index64 ? second : lo >> 31;
     return hi == 0 && lo >= 0 && lo < p.N ? lo : -1;
 }
 __device__ __forceinline__ int div_A(const CatArgs& p, int q) {
@@ -73,8 +73,10 @@ __global__ __launch_bounds__(NT, E * IT > 32 ? 4 : 8) void k_cat_rows(CatArgs p)
     double* terms = reinterpret_cast<double*>(seg + (size_t)RB * p.A);          // [RB][3]
     float* row_g = reinterpret_cast<float*>(terms + RB * 3);                    // [RB] upstream gradient
     float* row_in = row_g + RB;                                                 // [RB][3] = logp_old, adv, logp_ref
-    const T* logits = static_cast<const T*>(p.logits);
-    T* dlogits = static_cast<T*>(p.dlogits);
+    // (a block's rows span less than 2^31 bytes: 32-bit offsets from its first)
+    const T* logits = static_cast<const T*>(p.logits) + row0 * p.ld;
+    T* dlogits = static_cast<T*>(p.dlogits) + row0 * p.ldd;
+    const int ld = (int)p.ld, ldd = (int)p.ldd;
     // half of the exponentials wait in LDS while the heads run: their 64-bit arithmetic needs the registers
     float* parked = row_in + RB * 3;                                            // [IT / 2 * E][NT]
     const bool weighted = MODE == CAT_PPO && p.head.weight;
@@ -85,8 +87,9 @@ __global__ __launch_bounds__(NT, E * IT > 32 ? 4 : 8) void k_cat_rows(CatArgs p)
     auto segment_at = [&](int q, float w) {
         q = q < nseg ? q : nseg - 1;
         const int r = div_A(p, q), a = q - r * p.A;
-        return logits + (row0 + (w == 0.f ? 0 : r)) * p.ld + (size_t)a * p.N;
+        return logits + (unsigned)((w == 0.f ? 0 : r) * ld + a * p.N);
     };
+    const bool whole = p.N % ln.V == 0;          // packs belong to their lane entirely or not at all
     // one segment: exponentials, m, s
     auto softmax_of = [&](const T (&raw)[E], float (&x)[E], float& m, float& s) {
         m = -INFINITY;
@@ -97,11 +100,20 @@ __global__ __launch_bounds__(NT, E * IT > 32 ? 4 : 8) void k_cat_rows(CatArgs p)
         }
         m = group_max<G>(m);
         if (m == -INFINITY) m = 0.f;
-        s = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            x[e] = exp_below_exact(x[e], m);
-            s += ln.own(e) ? x[e] : 0.f;
+        for (int e = 0; e < E; ++e) x[e] = exp_below_exact(x[e], m);
+        s = 0.f;
+        if (whole) {
+#pragma unroll
+            for (int u = 0; u < ln.U; ++u) {
+                float t = x[u * ln.V];
+#pragma unroll
+                for (int v = 1; v < ln.V; ++v) t += x[u * ln.V + v];
+                s += ln.has(u) ? t : 0.f;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) s += ln.own(e) ? x[e] : 0.f;
         }
         s = group_sum<G>(s);
     };
@@ -110,7 +122,7 @@ __global__ __launch_bounds__(NT, E * IT > 32 ? 4 : 8) void k_cat_rows(CatArgs p)
         const int r = div_A(p, q), a = q - r * p.A;
         const bool live = k >= 0 && s != 0.f && g != 0.f;
         const float gi = g * (1.f / s);
-        T* d = dlogits + (row0 + r) * p.ldd + (size_t)a * p.N;
+        T* d = dlogits + (unsigned)(r * ldd + a * p.N);
         T o[E];
         if (MODE == CAT_BWD && p.accumulate) {
             if (!live) return;
@@ -599,6 +611,8 @@ static int lanes_per_row(int A) { return A <= 2 ? 1 : A <= 8 ? 4 : A <= 64 ? 16 
 
 template <typename T, int MODE, int G, int E, int IT, int NT>
 static int launch_rows(CatArgs p, int rb, hipStream_t st) {
+    const long long widest = p.ld > p.ldd ? p.ld : p.ldd;
+    while (rb > 1 && (long long)rb * widest * (long long)sizeof(T) >= (1ll << 31)) rb = (rb + 1) / 2;
     const long long blocks = ((long long)p.B + rb - 1) / rb;
     if (blocks > (long long)MAX_BLOCKS) return -1;
     p.rows_per_block = rb;

@@ -436,7 +436,10 @@ __global__ __launch_bounds__(BAL_NT) void k_bal_stats(BalArgs p) {
         const float ms = m == -INFINITY ? 0.f : m;
         float ex[E], s = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) { ex[e] = exp_below(x[e], ms); s += ex[e]; }
+        for (int e = 0; e < E; ++e) {
+            ex[e] = sizeof(T) == 4 ? exp_below_exact(x[e], ms) : exp_below(x[e], ms);
+            s += ex[e];
+        }
         s = group_sum<G>(s);
         const float inv = s == 0.f ? 0.f : 1.f / s;
 #pragma unroll
@@ -627,7 +630,7 @@ __global__ __launch_bounds__(BAL_NT) void k_bal_grad(BalArgs p) {
         float s = 0.f, d = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            x[e] = exp_below(x[e], m);
+            x[e] = sizeof(T) == 4 ? exp_below_exact(x[e], m) : exp_below(x[e], m);
             const float own = FULL || ln.own(e) ? x[e] : 0.f;
             s += own;
             d = __builtin_fmaf(own, f[e], d);

@@ -533,9 +533,20 @@ _LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _HERE = contextlib.nullcontext()
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _on(device):
     """the device of the tensors, where it is not the current one already"""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == _current_device() else torch.cuda.device(device)
+
+
+def _raw_stream(device):
+    """handle of the current stream of `device` (which is the current device by now)"""
+    try:
+        return torch._C._cuda_getCurrentRawStream(device.index)
+    except AttributeError:
+        return torch.cuda.current_stream(device).cuda_stream
 
 
 def _rows(t, n, device, name):
@@ -624,7 +635,7 @@ def categorical_logprob_fwd(logits, index, out=None):
     with _on(dev):
         ws = _scratch(lib.pfpn_categorical_workspace_bytes(B, A, N) if N > 1024 else 0, dev)
         _lib.check(lib.pfpn_categorical_logprob_fwd(pl, dt, ld, pi, i64, B, A, N, po, ws.data_ptr() if ws is not None else None,
-                                                    ws.numel() if ws is not None else 0, _stream()),
+                                                    ws.numel() if ws is not None else 0, _raw_stream(dev)),
                    "pfpn_categorical_logprob_fwd")
     return logp
 
@@ -644,7 +655,7 @@ def categorical_logprob_bwd(logits, index, dlogp, dlogits=None):
         ws = _scratch(lib.pfpn_categorical_workspace_bytes(B, A, N) if N > 1024 else 0, dev)
         _lib.check(lib.pfpn_categorical_logprob_bwd(pl, dt, ld, pi, i64, pg, B, A, N, int(acc), pd, ldd,
                                                     ws.data_ptr() if ws is not None else None,
-                                                    ws.numel() if ws is not None else 0, _stream()),
+                                                    ws.numel() if ws is not None else 0, _raw_stream(dev)),
                    "pfpn_categorical_logprob_bwd")
     return dlogits
 
@@ -686,7 +697,7 @@ def categorical_ppo_fwd_bwd(logits, index, logp_old, adv, logp_ref=None, weight=
     with _on(dev):
         ws = _scratch(lib.pfpn_categorical_workspace_bytes(B, A, N), dev)
         _lib.check(lib.pfpn_categorical_ppo_fwd_bwd(pl, dt, ld, pi, i64, *head, B, A, N, lo, hi, float(kl_coef), po, pd, ldd, p4,
-                                                    ws.data_ptr(), ws.numel(), _stream()), "pfpn_categorical_ppo_fwd_bwd")
+                                                    ws.data_ptr(), ws.numel(), _raw_stream(dev)), "pfpn_categorical_ppo_fwd_bwd")
     return out
 
 
@@ -709,7 +720,7 @@ def policy_kl_loss(logp, logp_old, adv, logp_ref=None, weight=None, stats=None, 
     lib = _lib.load()
     with _on(dev):
         ws = _scratch(lib.pfpn_policy_kl_workspace_bytes(n), dev)
-        _lib.check(lib.pfpn_policy_kl_loss(pl, *head, n, lo, hi, float(kl_coef), pd, p4, ws.data_ptr(), ws.numel(), _stream()),
+        _lib.check(lib.pfpn_policy_kl_loss(pl, *head, n, lo, hi, float(kl_coef), pd, p4, ws.data_ptr(), ws.numel(), _raw_stream(dev)),
                    "pfpn_policy_kl_loss")
     return dlogp, loss4
 
@@ -750,7 +761,7 @@ def preference_loss(logp, offsets, logp_ref=None, weight=None, beta=0.1, label_s
         ws = _scratch(lib.pfpn_preference_workspace_bytes(P, T), dev)
         _lib.check(lib.pfpn_preference_loss(pl, pr, pw, offsets.data_ptr(), P, T, float(beta), float(label_smoothing),
                                             _PREFERENCE_KINDS[kind], dlogp.data_ptr(), margin.data_ptr(), loss3.data_ptr(),
-                                            ws.data_ptr(), ws.numel(), _stream()), "pfpn_preference_loss")
+                                            ws.data_ptr(), ws.numel(), _raw_stream(dev)), "pfpn_preference_loss")
     return dlogp, margin, loss3
 
 
@@ -786,7 +797,7 @@ def balance_loss(logits, topk=1, coef=1.0, mask=None, dlogits=None, out=None):
     with _on(dev):
         ws = _scratch(lib.pfpn_balance_workspace_bytes(R, A, N), dev)
         _lib.check(lib.pfpn_balance_loss(pl, dt, ld, pm, R, A, N, topk, float(coef), int(acc), loss.data_ptr(), counts.data_ptr(),
-                                         mean_prob.data_ptr(), pd, ldd, ws.data_ptr(), ws.numel(), _stream()),
+                                         mean_prob.data_ptr(), pd, ldd, ws.data_ptr(), ws.numel(), _raw_stream(dev)),
                    "pfpn_balance_loss")
     return loss, counts, mean_prob, dlogits
 
