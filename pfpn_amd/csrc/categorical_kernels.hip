@@ -13,12 +13,6 @@ namespace pfpn {
 // The same loss on log-probs that come from elsewhere (the particle mixture's own density): one pass over [n] vectors.
 // ---------------------------------------------------------------------------------------------------------------------
 // Four rows a load, from any alignment.  One block (n <= 4096) finishes the sums itself.
-__device__ __forceinline__ void write_loss4(const double* sums, double kl_coef, float* loss4) {
-    loss4[0] = (float)(sums[0] + kl_coef * sums[1]);
-    loss4[1] = (float)sums[0];
-    loss4[2] = (float)sums[1];
-    loss4[3] = (float)sums[2];
-}
 constexpr long long ROWS_SMALL = 4096;
 
 template <int NT>
@@ -91,13 +85,14 @@ int cat_splits(int B, int A, int N) {
 }
 
 template <int MODE>
-static int run_typed(const CatArgs& p, int dtype, void* ws, size_t ws_bytes, float* loss4, void* stream) {
+static int run_typed(CatArgs p, int dtype, void* ws, size_t ws_bytes, float* loss4, void* stream) {
     hipStream_t st = (hipStream_t)stream;
+    p.loss4 = loss4;
     size_t nparts = 0;
     const int rc = dtype == DT_F32 ? run_cat<float, MODE>(p, ws, ws_bytes, &nparts, st)
                  : dtype == DT_BF16 ? run_cat<bf16_t, MODE>(p, ws, ws_bytes, &nparts, st)
                                     : run_cat<f16_t, MODE>(p, ws, ws_bytes, &nparts, st);
-    if (rc != PFPN_OK || MODE != CAT_PPO) return rc;
+    if (rc != PFPN_OK || MODE != CAT_PPO || nparts == 0) return rc;
     hipLaunchKernelGGL(k_policy_finish, dim3(1), dim3(1024), 0, st, (const double*)ws, nparts, p.head.kl_coef, loss4);
     PFPN_CHECK_LAUNCH();
     return PFPN_OK;
@@ -110,7 +105,7 @@ static bool bad_shape(const void* logits, int dtype, long long ld, const void* i
 static bool bad_head(const HeadArgs& h) {
     return !h.logp_old || !h.adv || !(h.clip_lo <= 1.0) || !(h.clip_hi >= 1.0) || (h.kl_coef != 0.0 && !h.logp_ref);
 }
-static int policy_row_blocks(long long n) { return (int)(n / 1024 + 1 < 2048 ? n / 1024 + 1 : 2048); }
+static int policy_row_blocks(long long n) { return (int)(n / 2048 + 1 < 2048 ? n / 2048 + 1 : 2048); }
 
 }  // namespace pfpn
 

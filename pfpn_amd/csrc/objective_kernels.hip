@@ -90,12 +90,14 @@ __device__ __forceinline__ double pair_head(const PrefArgs& p, int pair, double 
     const double m = p.beta * delta;
     double loss, slope;
     if (p.kind == 0) {
-        // log sigma(m) = -softplus(-m); both halves from ONE exponential of -|m|
-        const double z = exp(-fabs(m)), l = log1p(z);
-        const double good = m >= 0 ? 1.0 / (1.0 + z) : z / (1.0 + z), bad = m >= 0 ? z / (1.0 + z) : 1.0 / (1.0 + z);
-        const double sp_neg = l + (m < 0 ? -m : 0.0), sp_pos = l + (m > 0 ? m : 0.0);
-        loss = (1.0 - p.smoothing) * sp_neg + p.smoothing * sp_pos;
-        slope = p.beta * (p.smoothing * good - (1.0 - p.smoothing) * bad);
+        // log sigma(m) = -softplus(-m); both halves from ONE exponential of -|m|, in 32 bits (off by a few 2^-24 of themselves)
+        const float e = (float)p.smoothing, am = fabsf((float)m);
+        const float z = expf(-am), l = log1pf(z), near = 1.f / (1.f + z), far = z * near;
+        const float good = m >= 0 ? near : far, bad = m >= 0 ? far : near;
+        const float sp_neg = l + (m < 0 ? am : 0.f), sp_pos = l + (m > 0 ? am : 0.f);
+        loss = (1.f - e) * sp_neg + e * sp_pos;
+        slope = p.beta * (double)(e * good - (1.f - e) * bad);
+        if (m != m) { loss = m; slope = m; }
     } else {
         const double u = delta - 0.5 / p.beta;
         loss = u * u;

@@ -584,12 +584,13 @@ def _logit_rows(t, name="logits"):
 
 
 def _index(t, logits, name="index"):
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in (torch.int32, torch.int64) and t.is_contiguous()):
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.is_contiguous() and
+            (t.dtype is torch.int32 or t.dtype is torch.int64)):
         raise ValueError("%s must be a contiguous int32 or int64 CUDA tensor" % name)
     if t.shape != logits.shape[:-1] or t.device != logits.device:
         raise ValueError("%s has shape %s on %s, expected %s on %s" % (name, tuple(t.shape), t.device,
                                                                        tuple(logits.shape[:-1]), logits.device))
-    return t.data_ptr(), int(t.dtype == torch.int64)
+    return t.data_ptr(), int(t.dtype is torch.int64)
 
 
 def _logit_grad(dlogits, logits):
