@@ -270,22 +270,42 @@ __global__ __launch_bounds__(NT, E * IT > 32 ? 4 : 8) void k_cat_rows(CatArgs p)
 // thread, raw), so the logits are read once whatever their length: one pass finds {m, s}, the gradient is formed from the registers.
 // For A = 1 (a token row) the loss head sits in between, computed by every thread alike (no second barrier).
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename T>
-__device__ __forceinline__ void block_softmax(float m, float s, float* red, int nw, float& M, float& S) {
-    // (m, s) of a wave, wave-uniform -> of the block
+template <int NW>
+__device__ __forceinline__ void block_softmax(float m, float s, float* red, float& M, float& S) {
+    // (m, s) of a wave, wave-uniform -> of the block: a lane a wave
     if ((threadIdx.x & 63) == 0) {
         red[(threadIdx.x >> 6) * 2] = m;
         red[(threadIdx.x >> 6) * 2 + 1] = s;
     }
     __syncthreads();
-    M = red[0];
-    S = red[1];
-    for (int i = 1; i < nw; ++i) join_softmax(M, S, red[i * 2], red[i * 2 + 1]);
+    const int i = threadIdx.x & (NW - 1);
+    const float mi = red[i * 2], si = red[i * 2 + 1];
+    M = group_max<NW>(mi);
     if (M == -INFINITY) M = 0.f;
+    S = group_sum<NW>(si * exp_below(mi, M));
 }
 
-// -g p of one logit, as v_exp_f32 of ONE argument where the output has 16 bits: log2 |g / s| joins the exponent (its rounding,
-// 2^-24 of an argument of some tens, is far under the output's half step); 32-bit outputs multiply instead
+// exp(x - m) as v_exp_f32 of ONE fma, x log2(e) - c: what rounding c = m log2(e) does is common to all terms, `left` (in powers of two).
+// Within |m| <= 256: beyond, and where m is infinite, the difference is formed first.
+constexpr float EXP_NEAR = 256.f;
+struct NearExp {
+    float c, left;
+    __device__ __forceinline__ explicit NearExp(float m) : c(-m * PFPN_LOG2E), left(__builtin_fmaf(m, PFPN_LOG2E, c)) {}
+    __device__ __forceinline__ float operator()(float x) const {
+        return __builtin_amdgcn_exp2f(__builtin_fmaf(x, PFPN_LOG2E, c));
+    }
+};
+
+// |g| p of one logit of a 16-bit gradient: log2 |g / s| joins the exponent too (rounded at 2^-24 of some hundreds, far under
+// the output's half step)
+struct NearProb {
+    float c;
+    __device__ __forceinline__ NearProb(float m, float log_scale) : c(__builtin_fmaf(-m, PFPN_LOG2E, log_scale)) {}
+    __device__ __forceinline__ float operator()(float x) const {
+        return __builtin_amdgcn_exp2f(__builtin_fmaf(x, PFPN_LOG2E, c));
+    }
+};
+// -g p of one logit, any type, any m
 template <typename T>
 struct NegProb {
     float m, scale, log_scale;
@@ -346,29 +366,42 @@ __global__ __launch_bounds__(NT, H > 8 ? 4 : 8) void k_cat_long_held(CatArgs p) 
         if ((h * NT + tid) * V >= full) raw[h].fill(closed_logits<T>());
     if (last < N) tail = to_f32(l[last]);
     const float xk = k >= 0 ? to_f32(l[k]) : 0.f;
-    float m = tail;
+    HeldMax<T> top;
 #pragma unroll
     for (int h = 0; h < H; ++h) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) m = fmaxf(m, raw[h][i]);
+        for (int i = 0; i < raw[h].W; ++i) top.take(raw[h].w[i]);
         raw[h].forget();
     }
-    m = group_max<64>(m);
+    const float m = group_max<64>(fmaxf(tail, top.value()));
     const float mw = m == -INFINITY ? 0.f : m;
-    float s = exp_below(tail, mw);
+    const bool near = fabsf(mw) <= EXP_NEAR;        // (the same in the whole wave; false for a NaN)
+    const NearExp ne(mw);
+    float s = 0.f;
+    if (near) {
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-        if (h * NT * V < full) {
-            float t = 0.f;
+        for (int h = 0; h < H; ++h) {
+            if (h * NT * V < full) {
+                float t = ne(raw[h][0]);
 #pragma unroll
-            for (int i = 0; i < V; ++i) t += exp_below(raw[h][i], mw);
-            s += t;
+                for (int i = 1; i < V; ++i) t += ne(raw[h][i]);
+                s += t;
+            }
+            raw[h].forget();
         }
-        raw[h].forget();
+        s = (s + ne(tail)) * __builtin_amdgcn_exp2f(-ne.left);
+    } else {
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) s += exp_below(raw[h][i], mw);
+            raw[h].forget();
+        }
+        s += exp_below(tail, mw);
     }
     s = group_sum<64>(s);
     float M, S;
-    block_softmax<T>(m, s, red, NT / 64, M, S);
+    block_softmax<NT / 64>(m, s, red, M, S);
     if (MODE == CAT_FWD) {
         if (tid == 0) p.logp[b] = (float)token_logp(k, xk, M, S);
         return;
@@ -399,32 +432,56 @@ __global__ __launch_bounds__(NT, H > 8 ? 4 : 8) void k_cat_long_held(CatArgs p) 
         for (int i = 0; i < PARK * 4; ++i) raw[H - PARK + i / 4].w[i % 4] = parked[i * NT + tid];
     }
     const bool live = k >= 0 && S != 0.f && g != 0.f, acc = MODE == CAT_BWD && p.accumulate;
-    const NegProb<T> np(live ? M : 0.f, live ? g : 0.f, live ? 1.f / S : 0.f);
-    const float gk = live ? g - exp_below_exact(xk, M) * (g * (1.f / S)) : 0.f;
+    const float inv = live ? 1.f / S : 0.f;
+    const NegProb<T> np(live ? M : 0.f, live ? g : 0.f, inv);
+    const float gk = live ? g - exp_below_exact(xk, M) * (g * inv) : 0.f;
+    if (sizeof(T) == 2 && live && !acc && fabsf(M) <= EXP_NEAR) {
+        // the usual case of a 16-bit gradient: two instructions, a conversion of two and the sign of two an element
+        const NearProb pr(M, np.log_scale);
+        const uint32_t sign = np.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-        const int n = (h * NT + tid) * V;
-        if (n < full) {
-            float v[V];
-            T o[V];
+        for (int h = 0; h < H; ++h) {
+            const int n = (h * NT + tid) * V;
+            if (n < full) {
+                T o[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = 0.f;
-            if (live) {
+                for (int i = 0; i < V; i += 2) {
+                    const T a0 = from_f32<T>(pr(raw[h][i])), a1 = from_f32<T>(pr(raw[h][i + 1]));
+                    const uint32_t w = ((uint32_t)__builtin_bit_cast(typename Bits<T>::type, a0) |
+                                        (uint32_t)__builtin_bit_cast(typename Bits<T>::type, a1) << 16) | sign;
+                    o[i] = __builtin_bit_cast(T, (typename Bits<T>::type)w);
+                    o[i + 1] = __builtin_bit_cast(T, (typename Bits<T>::type)(w >> 16));
+                }
+                if ((unsigned)(k - n) < (unsigned)V) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) v[i] = np(raw[h][i]);
+                    for (int i = 0; i < V; ++i)
+                        if (n + i == k) o[i] = from_f32<T>(gk);
+                }
+                store_pack<T, V>(d + n, o, p.stream);
             }
-            if ((unsigned)(k - n) < (unsigned)V) {
+        }
+    } else {
 #pragma unroll
-                for (int i = 0; i < V; ++i) v[i] = n + i == k ? gk : v[i];
+        for (int h = 0; h < H; ++h) {
+            const int n = (h * NT + tid) * V;
+            if (n < full) {
+                float v[V];
+                T o[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[i] = live ? np(raw[h][i]) : 0.f;
+                if ((unsigned)(k - n) < (unsigned)V) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) v[i] = n + i == k ? gk : v[i];
+                }
+                if (acc) {
+                    load_pack<T, V>(d + n, o);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) v[i] += to_f32(o[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < V; ++i) o[i] = from_f32<T>(v[i]);
+                store_pack<T, V>(d + n, o, p.stream);
             }
-            if (acc) {
-                load_pack<T, V>(d + n, o);
-#pragma unroll
-                for (int i = 0; i < V; ++i) v[i] += to_f32(o[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < V; ++i) o[i] = from_f32<T>(v[i]);
-            store_pack<T, V>(d + n, o, p.stream);
         }
     }
     if (last < N) {
@@ -490,7 +547,7 @@ __global__ __launch_bounds__(LONG_NT) void k_cat_long_stats(CatArgs p, int split
     const float ms = mw == -INFINITY ? 0.f : mw;
     const float sw = group_sum<64>(s * exp_below(m, ms));
     float M, S;
-    block_softmax<T>(mw, sw, red, LONG_NT / 64, M, S);
+    block_softmax<LONG_NT / 64>(mw, sw, red, M, S);
     if (threadIdx.x == 0) {
         stats[(size_t)blockIdx.x * 2] = S == 0.f ? -INFINITY : M;
         stats[(size_t)blockIdx.x * 2 + 1] = S;

@@ -57,18 +57,10 @@ __global__ __launch_bounds__(NT) void k_policy_rows(const float* __restrict__ lo
 }
 
 // loss4 = {policy + c kl, policy, kl, clipped}: the blocks' sums in a fixed order
-__global__ __launch_bounds__(1024) void k_policy_finish(const double* __restrict__ part, size_t nparts, double kl_coef,
-                                                        float* __restrict__ loss4) {
-    __shared__ double red[3 * 16];
+__global__ __launch_bounds__(FINISH_NT) void k_policy_finish(const double* __restrict__ part, size_t nparts, double kl_coef,
+                                                             float* __restrict__ loss4) {
     __shared__ double out[3];
-    HeadTerms t = {0.0, 0.0, 0.0};
-    for (size_t i = threadIdx.x; i < nparts; i += 1024) {
-        t.policy += part[i * 3];
-        t.kl += part[i * 3 + 1];
-        t.clipped += part[i * 3 + 2];
-    }
-    block_terms(t, red, out);
-    __syncthreads();
+    sum_terms(part, nparts, out);
     if (threadIdx.x == 0) write_loss4(out, kl_coef, loss4);
 }
 
@@ -93,7 +85,7 @@ static int run_typed(CatArgs p, int dtype, void* ws, size_t ws_bytes, float* los
                  : dtype == DT_BF16 ? run_cat<bf16_t, MODE>(p, ws, ws_bytes, &nparts, st)
                                     : run_cat<f16_t, MODE>(p, ws, ws_bytes, &nparts, st);
     if (rc != PFPN_OK || MODE != CAT_PPO || nparts == 0) return rc;
-    hipLaunchKernelGGL(k_policy_finish, dim3(1), dim3(1024), 0, st, (const double*)ws, nparts, p.head.kl_coef, loss4);
+    hipLaunchKernelGGL(k_policy_finish, dim3(1), dim3(FINISH_NT), 0, st, (const double*)ws, nparts, p.head.kl_coef, loss4);
     PFPN_CHECK_LAUNCH();
     return PFPN_OK;
 }
@@ -177,7 +169,7 @@ int pfpn_policy_kl_loss(const float* logp, const float* logp_old, const float* a
     } else {
         const int blocks = policy_row_blocks(n);
         hipLaunchKernelGGL((k_policy_rows<256>), dim3(blocks), dim3(256), 0, st, logp, h, (size_t)n, dlogp, part, (float*)nullptr);
-        hipLaunchKernelGGL(k_policy_finish, dim3(1), dim3(1024), 0, st, (const double*)part, (size_t)blocks, kl_coef, loss4);
+        hipLaunchKernelGGL(k_policy_finish, dim3(1), dim3(FINISH_NT), 0, st, (const double*)part, (size_t)blocks, kl_coef, loss4);
     }
     PFPN_CHECK_LAUNCH();
     return PFPN_OK;

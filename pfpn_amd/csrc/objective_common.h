@@ -91,6 +91,31 @@ struct Held {
     }
 };
 
+// Running maximum of held logits: two 16-bit ones an instruction (bfloat16 as integers in the same order; a NaN may be passed
+// over here, it reaches the sum)
+template <typename T> struct HeldMax;
+template <> struct HeldMax<float> {
+    float m = -INFINITY;
+    __device__ __forceinline__ void take(uint32_t w) { m = fmaxf(m, __uint_as_float(w)); }
+    __device__ __forceinline__ float value() const { return m; }
+};
+template <> struct HeldMax<f16_t> {
+    typedef _Float16 Pair __attribute__((ext_vector_type(2)));
+    Pair m = {(_Float16)-INFINITY, (_Float16)-INFINITY};
+    __device__ __forceinline__ void take(uint32_t w) { m = __builtin_elementwise_max(m, __builtin_bit_cast(Pair, w)); }
+    __device__ __forceinline__ float value() const { return fmaxf((float)m[0], (float)m[1]); }
+};
+template <> struct HeldMax<bf16_t> {
+    typedef short Pair __attribute__((ext_vector_type(2)));
+    Pair m = {(short)0x8000, (short)0x8000};
+    static __device__ __forceinline__ Pair ordered(Pair v) { return v ^ ((v >> 15) & (short)0x7fff); }
+    __device__ __forceinline__ void take(uint32_t w) { m = __builtin_elementwise_max(m, ordered(__builtin_bit_cast(Pair, w))); }
+    __device__ __forceinline__ float value() const {
+        const Pair v = ordered(m);
+        return fmaxf(to_f32(bf16_t{(uint16_t)v[0]}), to_f32(bf16_t{(uint16_t)v[1]}));
+    }
+};
+
 // Reductions over aligned groups of G lanes (2 .. 64), every lane gets the result, no LDS round trip: quad_perm xor 1, xor 2,
 // row_half_mirror (quads of a half row), row_mirror (half rows), then gfx950's row / half-wave swaps.
 template <int CTRL>
@@ -265,6 +290,34 @@ __device__ __forceinline__ void block_terms(const HeadTerms& t, double* red, dou
         for (int i = 0; i < nw; ++i) s += red[i * 3 + threadIdx.x];
         part[threadIdx.x] = s;
     }
+}
+
+// n triples of terms added by one block of 15 waves, five a term, sixteen loads of a lane in flight; out[3] in LDS, fixed order
+constexpr int FINISH_NT = 960;
+__device__ __forceinline__ void sum_terms(const double* __restrict__ part, size_t n, double* out) {
+    constexpr int LANES = FINISH_NT / 3, DEEP = 16;
+    __shared__ double red[15];
+    const int wid = threadIdx.x >> 6, lane = threadIdx.x & 63, term = wid % 3;
+    double s = 0.0;
+    for (size_t i = (size_t)(wid / 3) * 64 + lane; i < n; i += LANES * DEEP) {
+        double t[DEEP];
+#pragma unroll
+        for (int k = 0; k < DEEP; ++k) {
+            const size_t j = i + LANES * k;
+            t[k] = part[(j < n ? j : i) * 3 + term];
+        }
+#pragma unroll
+        for (int k = 0; k < DEEP; ++k) s += i + LANES * k < n ? t[k] : 0.0;
+    }
+    s = wave_sum(s);
+    if (lane == 0) red[wid] = s;
+    __syncthreads();
+    if (threadIdx.x < 3) {
+        s = red[threadIdx.x];
+        for (int k = 1; k < 5; ++k) s += red[3 * k + threadIdx.x];
+        out[threadIdx.x] = s;
+    }
+    __syncthreads();
 }
 
 }  // namespace pfpn

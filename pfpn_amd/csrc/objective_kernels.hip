@@ -185,17 +185,9 @@ __global__ __launch_bounds__(256) void k_pref_grad(PrefArgs p) {
     span_grad(p, lo, hi, threadIdx.x, 256, (s & 1) ? -g : g);
 }
 
-__global__ __launch_bounds__(1024) void k_pref_finish(const double* __restrict__ terms, int P, float* __restrict__ loss3) {
-    __shared__ double red[3 * 16];
+__global__ __launch_bounds__(FINISH_NT) void k_pref_finish(const double* __restrict__ terms, int P, float* __restrict__ loss3) {
     __shared__ double out[3];
-    HeadTerms t = {0.0, 0.0, 0.0};
-    for (int i = threadIdx.x; i < P; i += 1024) {
-        t.policy += terms[(size_t)i * 3];
-        t.kl += terms[(size_t)i * 3 + 1];
-        t.clipped += terms[(size_t)i * 3 + 2];
-    }
-    block_terms(t, red, out);
-    __syncthreads();
+    sum_terms(terms, (size_t)P, out);
     if (threadIdx.x < 3) loss3[threadIdx.x] = (float)(out[threadIdx.x] / (double)P);
 }
 
@@ -780,7 +772,7 @@ int pfpn_preference_loss(const float* logp, const float* logp_ref, const float* 
         hipLaunchKernelGGL(k_pref_sums, dim3(blocks), dim3(256), 0, st, p);
         hipLaunchKernelGGL(k_pref_grad, dim3(blocks + outside), dim3(256), 0, st, p);
     }
-    hipLaunchKernelGGL(k_pref_finish, dim3(1), dim3(1024), 0, st, (const double*)p.terms, P, loss3);
+    hipLaunchKernelGGL(k_pref_finish, dim3(1), dim3(FINISH_NT), 0, st, (const double*)p.terms, P, loss3);
     PFPN_CHECK_LAUNCH();
     return PFPN_OK;
 }
