@@ -537,56 +537,62 @@ __global__ __launch_bounds__(BAL_NT) void k_bal_stats(BalArgs p) {
     }
 }
 
-// 32 columns x 32 lanes over the slabs, eight of them in flight a lane
+// 32 columns x 32 lanes over the slabs, sixteen of them in flight a lane; then 32 lanes a column
 __global__ __launch_bounds__(1024) void k_bal_reduce(BalArgs p) {
+    constexpr int DEEP = 16;
     __shared__ double rs[32][BAL_COLS + 1];
-    __shared__ uint32_t rn[32][BAL_COLS + 1];
-    __shared__ uint32_t v_all;
+    __shared__ uint32_t rn[32][BAL_COLS + 1], rv[16];
+    __shared__ double rt[16];
     const size_t AN = (size_t)p.A * p.N;
-    const int cl = threadIdx.x % BAL_COLS, kl = threadIdx.x / BAL_COLS;
-    const size_t col = (size_t)blockIdx.x * BAL_COLS + cl;
-    if (threadIdx.x == 0) v_all = 0;
-    __syncthreads();
+    const int cl = threadIdx.x % BAL_COLS, kl = threadIdx.x / BAL_COLS, lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    const size_t mine = (size_t)blockIdx.x * BAL_COLS + cl, col = mine < AN ? mine : AN - 1;
     uint32_t v = 0;
     for (int k = threadIdx.x; k < p.chunks; k += 1024) v += p.slab_v[k];
-    if (v) atomicAdd(&v_all, v);
     double s = 0.0;
     uint32_t n = 0;
-    if (col < AN) {
-        for (int k0 = kl; k0 < p.chunks; k0 += 32 * 8) {
-            float fp[8];
-            uint32_t fn[8];
+    for (int k0 = kl; k0 < p.chunks; k0 += 32 * DEEP) {
+        float fp[DEEP];
+        uint32_t fn[DEEP];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int k = k0 + 32 * i < p.chunks ? k0 + 32 * i : kl;
-                fp[i] = p.slab_p[(size_t)k * AN + col];
-                fn[i] = p.slab_n[(size_t)k * AN + col];
-            }
+        for (int i = 0; i < DEEP; ++i) {
+            const int k = k0 + 32 * i < p.chunks ? k0 + 32 * i : kl;
+            fp[i] = p.slab_p[(size_t)k * AN + col];
+            fn[i] = p.slab_n[(size_t)k * AN + col];
+        }
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (k0 + 32 * i < p.chunks) { s += (double)fp[i]; n += fn[i]; }
+        for (int i = 0; i < DEEP; ++i) {
+            const bool on = k0 + 32 * i < p.chunks;
+            s += on ? (double)fp[i] : 0.0;
+            n += on ? fn[i] : 0u;
         }
     }
     rs[kl][cl] = s;
     rn[kl][cl] = n;
+    v = group_add<64>(v);
+    if (lane == 0) rv[wid] = v;
     __syncthreads();
-    if (threadIdx.x < 64) {
-        double term = 0.0;
-        if (threadIdx.x < BAL_COLS) {
-            s = 0.0;
-            n = 0;
-            for (int i = 0; i < 32; ++i) { s += rs[i][cl]; n += rn[i][cl]; }
-            const double inv_v = v_all ? 1.0 / (double)v_all : 0.0;
-            const double mean = s * inv_v, share = (double)n * inv_v / p.K;
-            if (col < AN) {
-                p.mean_prob[col] = (float)mean;
-                p.counts[col] = (int)n;
-                p.f[col] = (float)(p.scale * inv_v * share);
-                term = share * mean;
-            }
-        }
-        term = wave_sum(term);
-        if (threadIdx.x == 0) p.terms[blockIdx.x] = term;
+    const int c2 = threadIdx.x / 32, k2 = threadIdx.x % 32;         // (a column by half a wave)
+    const size_t out = (size_t)blockIdx.x * BAL_COLS + c2;
+    s = rs[k2][c2];
+    n = group_add<32>(rn[k2][c2]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor(s, o, 64);
+    const uint32_t rows = group_add<16>(rv[threadIdx.x & 15]);
+    const double inv_v = rows ? 1.0 / (double)rows : 0.0;
+    const double mean = s * inv_v, share = (double)n * inv_v / p.K;
+    if (k2 == 0 && out < AN) {
+        p.mean_prob[out] = (float)mean;
+        p.counts[out] = (int)n;
+        p.f[out] = (float)(p.scale * inv_v * share);
+    }
+    double term = out < AN ? share * mean : 0.0;                    // (the same in a column's lanes)
+    term += __shfl_xor(term, 32, 64);
+    if (lane == 0) rt[wid] = term;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double t = 0.0;
+        for (int i = 0; i < 16; ++i) t += rt[i];
+        p.terms[blockIdx.x] = t;
     }
 }
 
