@@ -232,7 +232,8 @@ size_t pfpn_categorical_workspace_bytes(int B, int A, int N);
  * reference networks/utils.py:187-194). */
 int pfpn_categorical_logprob_fwd(const void* logits, int dtype, long long row_stride, const void* index, int index64,
                                  int B, int A, int N, float* logp, void* workspace, size_t workspace_bytes, void* stream);
-/* dlogits[b,a,n] (+)= dlogp[b] (1[n = index] - softmax_n); a row with dlogp 0 is not read. */
+/* dlogits[b,a,n] (+)= dlogp[b] (1[n = index] - softmax_n); a row with dlogp 0 gets zeros (accumulate: is left alone) whatever its
+ * logits hold. */
 int pfpn_categorical_logprob_bwd(const void* logits, int dtype, long long row_stride, const void* index, int index64,
                                  const float* dlogp, int B, int A, int N, int accumulate, void* dlogits,
                                  long long grad_stride, void* workspace, size_t workspace_bytes, void* stream);
@@ -240,8 +241,8 @@ int pfpn_categorical_logprob_bwd(const void* logits, int dtype, long long row_st
  * categorical log-probs, plus the sampled KL term to a reference policy):
  *   a = clip((adv - mean) rstd) (adv_stats NULL: adv itself), r = exp(logp - logp_old), d = logp_ref - logp,
  *   loss = sum_b w_b (-min(r a, clip(r, 1 - clip_eps_low, 1 + clip_eps_high) a) + kl_coef (exp(d) - 1 - d)).
- * logp_ref optional (NULL: no KL term, kl_coef must be 0); weight [B] optional (NULL: 1/B each) -- a row of weight 0 is not read
- * (whatever it holds), its logp and gradient are 0.  loss4 = {loss, sum w policy term, sum w kl, sum of w where the clip binds}. */
+ * logp_ref optional (NULL: no KL term, kl_coef must be 0); weight [B] optional (NULL: 1/B each) -- a row of weight 0 does not count
+ * whatever it holds, its logp and gradient are 0.  An impossible choice (logp -inf) makes the KL term infinite.  loss4 = {loss, sum w policy term, sum w kl, sum of w where the clip binds}. */
 int pfpn_categorical_ppo_fwd_bwd(const void* logits, int dtype, long long row_stride, const void* index, int index64,
                                  const float* logp_old, const float* adv, const float* logp_ref, const float* weight,
                                  const float* adv_stats, int B, int A, int N, double clip_eps_low, double clip_eps_high,
@@ -266,7 +267,7 @@ int pfpn_preference_loss(const float* logp, const float* logp_ref, const float* 
  * them: reference a2c.py:346-365).  Over the V rows that mask (uint8 [R], optional) leaves: counts[a,n] = rows whose topk largest
  * logits hold n (equal ones: lowest index first; -inf never), f = counts / (topk V), mean_prob = mean softmax,
  *   loss = coef N / A sum_{a,n} f mean_prob (>= coef, = coef when balanced), dlogits (+)= coef N / (A V) p_n (f_n - sum_m f_m p_m).
- * Masked rows are not read, their gradient is 0 (accumulate: left alone).  N <= 1024, A <= 4096, topk <= min(N, 64). */
+ * Masked rows do not count whatever they hold, their gradient is 0 (accumulate: left alone).  N <= 1024, A <= 4096, topk <= min(N, 64). */
 size_t pfpn_balance_workspace_bytes(int R, int A, int N);
 int pfpn_balance_loss(const void* logits, int dtype, long long row_stride, const uint8_t* mask, int R, int A, int N, int topk,
                       double coef, int accumulate, float* loss, int32_t* counts, float* mean_prob, void* dlogits,

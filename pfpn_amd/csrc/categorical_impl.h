@@ -36,7 +36,7 @@ __device__ __forceinline__ void write_loss4(const double* sums, double kl_coef, 
 
 constexpr int CAT_MAX_A = 4096, CAT_MAX_N = 1 << 30, CAT_SHORT_N = 1024;
 constexpr int CAT_MAX_SPLITS = 64;              // pieces of a long axis: one wave joins them
-constexpr size_t MAX_BLOCKS = 1u << 22;         // blocks * threads of one launch stay under 2^32
+constexpr size_t MAX_BLOCKS = (1u << 22) - 1;   // blocks * threads of one launch stay under 2^32
 
 // one call for logits of type T; *nparts: the blocks that left loss terms (CAT_PPO)
 template <typename T, int MODE>
@@ -268,7 +268,7 @@ __global__ __launch_bounds__(NT, E * IT > 32 ? 4 : 8) void k_cat_rows(CatArgs p)
 // ---------------------------------------------------------------------------------------------------------------------
 // Long axes (N > 1024), enough rows to fill the chip: a block owns a segment and keeps ALL of it in registers (H wide loads a
 // thread, raw), so the logits are read once whatever their length: one pass finds {m, s}, the gradient is formed from the registers.
-// For A = 1 (a token row) the loss head sits in between, computed by every thread alike (no second barrier).
+// For A = 1 (a token row) the loss head sits in between, run by one wave.
 // ---------------------------------------------------------------------------------------------------------------------
 template <int NW>
 __device__ __forceinline__ void block_softmax(float m, float s, float* red, float& M, float& S) {
@@ -572,64 +572,60 @@ __device__ __forceinline__ double segment_logp(const CatArgs& p, size_t b, int a
     return (double)x - (double)m - log((double)s);
 }
 
-// the joint log-prob of row b by a block: a wave per choice, in turn; {m, s} of choice `own_a` into own[0..1]
-template <typename T>
-__device__ __forceinline__ double row_logp(const CatArgs& p, size_t b, int splits, const float* stats, double* red, int own_a,
-                                           float* own) {
+// a block a row: its joint log-prob (a wave per choice, in turn) and, CAT_PPO, its upstream gradient and loss terms
+template <typename T, int MODE>
+__global__ __launch_bounds__(LONG_NT) void k_cat_long_rows(CatArgs p, int splits, const float* stats, float* row_g) {
+    __shared__ double red[LONG_NT / 64];
+    const size_t b = blockIdx.x;
     const int wid = threadIdx.x >> 6, nw = blockDim.x >> 6;
+    const bool on = MODE != CAT_PPO || row_weight(p, b) != 0.0;
     double lp = 0.0;
-    for (int c = wid; c < p.A; c += nw) {
+    for (int c = wid; on && c < p.A; c += nw) {
         float m, s;
         join_pieces(stats + (b * p.A + c) * splits * 2, splits, m, s);
-        if (c == own_a && (threadIdx.x & 63) == 0) { own[0] = m; own[1] = s; }
         lp += segment_logp<T>(p, b, c, m, s);
     }
     if ((threadIdx.x & 63) == 0) red[wid] = lp;
     __syncthreads();
-    lp = 0.0;
-    for (int i = 0; i < nw; ++i) lp += red[i];
-    return lp;
+    if (threadIdx.x == 0) {
+        lp = 0.0;
+        for (int i = 0; i < nw; ++i) lp += red[i];
+        p.logp[b] = (float)lp;
+        if (MODE == CAT_PPO) {
+            HeadTerms t = {0.0, 0.0, 0.0};
+            row_g[b] = on ? (float)policy_head(lp, head_row(p.head, b), p.head, t) : 0.f;
+            p.part[b * 3] = t.policy;
+            p.part[b * 3 + 1] = t.kl;
+            p.part[b * 3 + 2] = t.clipped;
+        }
+    }
 }
 
-template <typename T>
-__global__ __launch_bounds__(LONG_NT) void k_cat_long_logp(CatArgs p, int splits, const float* stats) {
-    __shared__ double red[LONG_NT / 64];
-    const double lp = row_logp<T>(p, blockIdx.x, splits, stats, red, -1, nullptr);
-    if (threadIdx.x == 0) p.logp[blockIdx.x] = (float)lp;
-}
-
+// MODE CAT_PPO: one choice a row, every wave joins and runs its head; CAT_BWD: the upstream gradient of the row is p.dlogp's
 template <typename T, int MODE>
 __global__ __launch_bounds__(LONG_NT) void k_cat_long_grad(CatArgs p, int splits, const float* stats) {
     constexpr int V = 16 / sizeof(T);
-    __shared__ double red[LONG_NT / 64];
-    __shared__ float own[2];                 // m, s of this segment
     const size_t s_id = blockIdx.x / splits;
     const int piece = blockIdx.x % splits;
     const size_t b = s_id / p.A;
     const int a = (int)(s_id % p.A);
     const int k = chosen_in(p, s_id);
-    HeadRow hr = {0.f, 0.f, 0.f, 1.0};
-    if (MODE == CAT_PPO) hr = head_row(p.head, b);
     float m = 0.f, s = 0.f, g = MODE == CAT_BWD ? p.dlogp[b] : 0.f;
-    const bool on = MODE == CAT_PPO ? hr.w != 0.0 : g != 0.f;
+    const bool on = MODE == CAT_PPO ? row_weight(p, b) != 0.0 : g != 0.f;
+    if (on) join_pieces(stats + s_id * splits * 2, splits, m, s);
     if (MODE == CAT_PPO) {
-        const bool first = piece == 0 && a == 0 && threadIdx.x == 0;
         HeadTerms t = {0.0, 0.0, 0.0};
         double lp = 0.0;
         if (on) {
-            lp = row_logp<T>(p, b, splits, stats, red, a, own);
-            g = (float)policy_head(lp, hr, p.head, t);
-            m = own[0];
-            s = own[1];
+            lp = segment_logp<T>(p, b, 0, m, s);
+            g = (float)policy_head(lp, head_row(p.head, b), p.head, t);
         }
-        if (first) {
+        if (piece == 0 && threadIdx.x == 0) {
             p.logp[b] = (float)lp;
             p.part[b * 3] = t.policy;
             p.part[b * 3 + 1] = t.kl;
             p.part[b * 3 + 2] = t.clipped;
         }
-    } else if (on) {
-        join_pieces(stats + s_id * splits * 2, splits, m, s);
     }
     int lo, hi;
     piece_of(p, splits, piece, V, lo, hi);
@@ -778,14 +774,20 @@ int run_cat(CatArgs p, void* ws, size_t ws_bytes, size_t* nparts, hipStream_t st
         return PFPN_OK;
     }
     const size_t pieces = segs * S;
-    if (!ws || ws_bytes < parts + pieces * 2 * sizeof(float)) return PFPN_ERR_WORKSPACE;
+    if (!ws || ws_bytes < parts + pieces * 2 * sizeof(float) + (MODE == CAT_PPO ? (size_t)p.B * sizeof(float) : 0))
+        return PFPN_ERR_WORKSPACE;
     float* stats = reinterpret_cast<float*>(static_cast<char*>(ws) + parts);
     hipLaunchKernelGGL((k_cat_long_stats<T>), dim3((unsigned)pieces), dim3(LONG_NT), 0, st, p, S, MODE, stats);
-    if (MODE == CAT_FWD)
-        hipLaunchKernelGGL((k_cat_long_logp<T>), dim3(p.B), dim3(p.A < 4 ? 64 : LONG_NT), 0, st, p, S, (const float*)stats);
-    else
-        hipLaunchKernelGGL((k_cat_long_grad<T, MODE == CAT_FWD ? CAT_BWD : MODE>), dim3((unsigned)pieces), dim3(LONG_NT), 0, st, p, S,
-                           (const float*)stats);
+    constexpr int ROWS = MODE == CAT_PPO ? CAT_PPO : CAT_FWD;
+    if (MODE == CAT_FWD || (MODE == CAT_PPO && p.A > 1)) {
+        float* row_g = stats + pieces * 2;
+        hipLaunchKernelGGL((k_cat_long_rows<T, ROWS>), dim3(p.B), dim3(p.A < 4 ? 64 : LONG_NT), 0, st, p, S, (const float*)stats, row_g);
+        p.dlogp = row_g;
+    }
+    if (MODE == CAT_PPO && p.A == 1)
+        hipLaunchKernelGGL((k_cat_long_grad<T, CAT_PPO>), dim3((unsigned)pieces), dim3(LONG_NT), 0, st, p, S, (const float*)stats);
+    else if (MODE != CAT_FWD)
+        hipLaunchKernelGGL((k_cat_long_grad<T, CAT_BWD>), dim3((unsigned)pieces), dim3(LONG_NT), 0, st, p, S, (const float*)stats);
     PFPN_CHECK_LAUNCH();
     return PFPN_OK;
 }

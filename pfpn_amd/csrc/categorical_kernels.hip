@@ -108,7 +108,7 @@ extern "C" {
 size_t pfpn_categorical_workspace_bytes(int B, int A, int N) {
     if (B < 1 || A < 1 || N < 1) return 0;
     const size_t parts = (size_t)B * 3 * sizeof(double);
-    return N <= CAT_SHORT_N ? parts : parts + (size_t)B * A * cat_splits(B, A, N) * 2 * sizeof(float);
+    return N <= CAT_SHORT_N ? parts : parts + (size_t)B * A * cat_splits(B, A, N) * 2 * sizeof(float) + (size_t)B * sizeof(float);
 }
 
 int pfpn_categorical_logprob_fwd(const void* logits, int dtype, long long row_stride, const void* index, int index64,
@@ -116,7 +116,7 @@ int pfpn_categorical_logprob_fwd(const void* logits, int dtype, long long row_st
     PFPN_BEGIN();
     if (bad_shape(logits, dtype, row_stride, index, B, A, N) || !logp) return PFPN_ERR_ARG;
     CatArgs p = {};
-    p.logits = logits; p.ld = row_stride; p.index = index; p.index64 = index64;
+    p.logits = logits; p.ld = row_stride; p.index = index; p.index64 = index64 != 0;
     p.B = B; p.A = A; p.N = N; p.logp = logp;
     return run_typed<CAT_FWD>(p, dtype, workspace, workspace_bytes, nullptr, stream);
 }
@@ -128,7 +128,7 @@ int pfpn_categorical_logprob_bwd(const void* logits, int dtype, long long row_st
     if (bad_shape(logits, dtype, row_stride, index, B, A, N) || !dlogp || !dlogits || grad_stride < (long long)A * N)
         return PFPN_ERR_ARG;
     CatArgs p = {};
-    p.logits = logits; p.ld = row_stride; p.index = index; p.index64 = index64;
+    p.logits = logits; p.ld = row_stride; p.index = index; p.index64 = index64 != 0;
     p.B = B; p.A = A; p.N = N; p.dlogp = dlogp; p.dlogits = dlogits; p.ldd = grad_stride; p.accumulate = accumulate;
     return run_typed<CAT_BWD>(p, dtype, workspace, workspace_bytes, nullptr, stream);
 }
@@ -145,7 +145,7 @@ int pfpn_categorical_ppo_fwd_bwd(const void* logits, int dtype, long long row_st
     if (bad_shape(logits, dtype, row_stride, index, B, A, N) || bad_head(p.head) || !logp || !dlogits || !loss4 ||
         grad_stride < (long long)A * N)
         return PFPN_ERR_ARG;
-    p.logits = logits; p.ld = row_stride; p.index = index; p.index64 = index64;
+    p.logits = logits; p.ld = row_stride; p.index = index; p.index64 = index64 != 0;
     p.B = B; p.A = A; p.N = N; p.logp = logp; p.dlogits = dlogits; p.ldd = grad_stride;
     return run_typed<CAT_PPO>(p, dtype, workspace, workspace_bytes, loss4, stream);
 }

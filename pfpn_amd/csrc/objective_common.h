@@ -255,7 +255,7 @@ __device__ __forceinline__ float kl_sample(float d, float& em1) {
         return kl;
     }
     em1 = expf(d) - 1.f;
-    return em1 - d;
+    return em1 == INFINITY ? em1 : em1 - d;         // (an impossible choice: infinite, not inf - inf)
 }
 
 // -> d loss / d logp of a row of weight != 0; its terms

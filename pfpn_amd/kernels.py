@@ -715,6 +715,8 @@ def policy_kl_loss(logp, logp_old, adv, logp_ref=None, weight=None, stats=None, 
     dlogp = torch.empty(n, dtype=torch.float32, device=dev) if dlogp is None else dlogp
     loss4 = torch.empty(4, dtype=torch.float32, device=dev) if loss4 is None else loss4
     pd, p4 = _rows(dlogp, n, dev, "dlogp"), _rows(loss4, 4, dev, "loss4")
+    if pd == pl and n:
+        raise ValueError("dlogp overlaps logp")
     if n == 0:
         loss4.zero_()
         return dlogp, loss4

@@ -12,7 +12,7 @@ TYPES = [torch.float32, torch.bfloat16, torch.float16]
 SHAPES = [(1, 1, 1), (1, 1, 2), (3, 2, 1), (1, 36, 35), (33, 36, 35), (257, 5, 8), (64, 3, 9), (33, 2, 17), (20, 7, 25), (19, 7, 33),
           (5, 130, 41), (7, 13, 64), (5, 3, 65), (5, 3, 96), (9, 4, 97), (9, 4, 128), (6, 2, 129), (6, 2, 192), (5, 3, 193), (5, 128, 256),
           (4, 2, 257), (4, 2, 512), (3, 2, 513), (3, 2, 1024), (2, 3, 1025), (5, 1, 4097), (1, 3, 8191), (3, 1, 50021), (1, 1, 128000),
-          (700, 1, 1500), (2, 4096, 3), (1025, 1, 37)]
+          (700, 1, 1500), (2, 4096, 3), (1025, 1, 37), (4, 36, 35), (9, 7, 1100), (2, 600, 1030), (3, 700, 300), (2100, 1, 300)]
 
 
 def make_logits(dev, B, A, N, dtype, pad=0, seed=0, closed=0.0, width=1.5):
@@ -135,6 +135,70 @@ def test_nan_logits_stay_in_their_row(dev, N):
     bad[2] = math.nan
     out = kernels.categorical_ppo_fwd_bwd(x, k, bad, bad, logp_ref=bad, weight=up, kl_coef=0.1)
     assert not any(t.isnan().any() for t in out.values()) and out["logp"][2] == 0 and not out["dlogits"][2].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,N", [(520, 1500), (513, 9000), (512, 20001), (3, 6000)])
+def test_long_rows_of_every_kind(dev, B, N, dtype):
+    """the rows a chip full of long ones may hold: nothing open, one open, all at the type's lowest value, large and equal, far from
+    zero, a NaN, no upstream gradient -- none of them touches another"""
+    from pfpn_amd import kernels
+    x, k, g = make_logits(dev, B, 1, N, dtype, pad=1, seed=N)
+    info = torch.finfo(dtype)
+    x[0] = -math.inf
+    x[1] = -math.inf
+    x[1, 0, N - 1], k[1] = 2.0, N - 1
+    x[2] = info.min
+    if B > 8:
+        x[3] = info.max
+        x[4] += 300.0                               # (beyond the near range of the exponent; 16-bit steps of 1/4 .. 2)
+        x[5] -= 2000.0
+        x[6, 0, 1:] = info.min
+        x[7, 0, N // 3] = math.nan
+        x[8, 0, N // 3], k[8] = -math.inf, N // 3
+    dlogp = torch.randn(B, device=dev, generator=g)
+    finite = torch.ones(B, dtype=torch.bool, device=dev)
+    want, bound = logprob(x, k)
+    got = kernels.categorical_logprob_fwd(x, k)
+    wg, bg = gradient(x, k, dlogp)
+    d = kernels.categorical_logprob_bwd(x, k, dlogp)
+    assert got[0] == -math.inf and not d[0].any()
+    if B > 8:
+        assert got[7].isnan() and d[7].isnan().all() and got[8] == -math.inf
+        finite[7] = False
+        off = dlogp.clone()
+        off[7] = 0.0
+        d0 = kernels.categorical_logprob_bwd(x, k, off)
+        assert not d0[7].any() and torch.equal(d0[finite], d[finite])
+    close(got[finite], want[finite], bound[finite], "logp")
+    close(d[finite], wg[finite], rounded(wg, bg, dtype)[finite], "dlogits")
+
+
+@pytest.mark.parametrize("shape", [(600, 1, 1500), (40, 1, 3000), (700, 2, 1100), (30, 5, 2000)])
+def test_rows_without_weight_may_hold_anything(dev, shape):
+    from pfpn_amd import kernels
+    x, k, g = make_logits(dev, *shape, torch.bfloat16, seed=2)
+    old, adv, ref, w = objective(dev, logprob(x, k)[0], g, True)
+    w[:3] = torch.tensor([0.5, 0.0, 0.25], device=dev)
+    a = kernels.categorical_ppo_fwd_bwd(x, k, old, adv, logp_ref=ref, weight=w, kl_coef=0.1)
+    gone = w == 0
+    x[gone], old[gone], adv[gone], ref[gone] = math.nan, math.nan, math.inf, -math.inf
+    b = kernels.categorical_ppo_fwd_bwd(x, k, old, adv, logp_ref=ref, weight=w, kl_coef=0.1)
+    assert all(torch.equal(a[n], b[n]) for n in a) and not a["dlogits"][gone].any() and not a["logp"][gone].any()
+    nothing = kernels.categorical_ppo_fwd_bwd(x, k, old, adv, logp_ref=ref, weight=torch.zeros_like(w), kl_coef=0.1)
+    assert not any(t.any() for t in nothing.values())
+
+
+def test_impossible_choice(dev):
+    """probability zero: log-prob -inf, ratio 0; without a KL term a finite loss, with one an infinite one"""
+    from pfpn_amd import kernels
+    x, k = torch.zeros(4, 2, 6, device=dev), torch.zeros(4, 2, dtype=torch.int32, device=dev)
+    x[1, 0, 0] = -math.inf
+    v = torch.full((4,), -3.5, device=dev)
+    out = kernels.categorical_ppo_fwd_bwd(x, k, v, torch.ones(4, device=dev))
+    assert out["logp"][1] == -math.inf and bool(torch.isfinite(out["loss4"]).all()) and not out["dlogits"][1].any()
+    out = kernels.categorical_ppo_fwd_bwd(x, k, v, torch.ones(4, device=dev), logp_ref=v, kl_coef=0.1)
+    assert out["loss4"][0] == math.inf and out["loss4"][2] == math.inf and bool(torch.isfinite(out["dlogits"][[0, 2, 3]]).all())
 
 
 # ---- clipped loss with a KL term ----------------------------------------------------------------------------------------------
@@ -398,7 +462,7 @@ def _together(kernels, x, k, old, adv, ref, w, offsets, mask):
     return [out["logp"], out["dlogits"], out["loss4"], bal[0], bal[1], bal[2], margin, l3, d2, d3, l4]
 
 
-@pytest.mark.parametrize("shape", [(64, 36, 35), (12, 1, 5000)])
+@pytest.mark.parametrize("shape", [(64, 36, 35), (12, 128, 256), (300, 1, 64), (12, 1, 5000), (530, 1, 2100), (11, 3, 1300)])
 def test_together_on_a_side_stream_and_replayed(dev, shape):
     from pfpn_amd import kernels
     B, A, N = shape
