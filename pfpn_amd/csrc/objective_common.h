@@ -155,6 +155,25 @@ __device__ __forceinline__ uint32_t group_min(uint32_t v) {
     return group_reduce<G>(v, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
 }
 
+// Sum over the lanes of a wave that stand at the same place of their groups of G (every lane gets it): rotations inside the rows of
+// 16, then the row and half-wave swaps.
+template <int G, typename F>
+__device__ __forceinline__ uint32_t across_groups(uint32_t v, F op) {
+    if (G < 16) v = op(v, lane_move<0x128>(v));
+    if (G < 8) v = op(v, lane_move<0x124>(v));
+    if (G < 4) v = op(v, lane_move<0x122>(v));
+    if (G < 2) v = op(v, lane_move<0x121>(v));
+    if (G < 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = op(r[0], r[1]);
+    }
+    if (G < 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = op(r[0], r[1]);
+    }
+    return v;
+}
+
 // exp(x - m): the difference first (exact where it matters: near the maximum), then ONE v_exp_f32
 __device__ __forceinline__ float exp_below(float x, float m) {
     return __builtin_amdgcn_exp2f((x - m) * PFPN_LOG2E);

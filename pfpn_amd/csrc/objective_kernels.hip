@@ -23,30 +23,39 @@ struct PrefArgs {
     int kind;                   // 0 logistic, 1 squared
     float* dlogp;
     float* margin;
-    double* sums;               // [2P][splits]
+    double* sums;               // [P][splits]
     double* terms;              // [P][3] = loss, margin > 0, margin
     int splits;
 };
 
-__device__ __forceinline__ void segment_of(const PrefArgs& p, int s, long long& lo, long long& hi) {
-    lo = p.offsets[s];
-    hi = p.offsets[s + 1];
-    lo = lo < 0 ? 0 : (lo > p.T ? p.T : lo);
-    hi = hi < lo ? lo : (hi > p.T ? p.T : hi);
+// A pair's two segments lie side by side: rows [lo, mid) count for it, [mid, hi) against it.  Bounds are clamped to the vectors
+// (and to ascend), so that nothing outside is touched whatever they hold.
+struct PairRows {
+    long long lo, mid, hi;
+};
+__device__ __forceinline__ long long clamped(long long v, long long lo, long long hi) { return v < lo ? lo : (v > hi ? hi : v); }
+__device__ __forceinline__ PairRows rows_of_pair(const PrefArgs& p, int pair) {
+    const long long* o = p.offsets + 2 * (size_t)pair;
+    PairRows r;
+    const long long a = o[0], b = o[1], c = o[2];
+    r.lo = clamped(a, 0, p.T);
+    r.mid = clamped(b, r.lo, p.T);
+    r.hi = clamped(c, r.mid, p.T);
+    return r;
 }
-__device__ __forceinline__ void slice_of(const PrefArgs& p, int s, int part, long long& lo, long long& hi) {
-    long long a, b;
-    segment_of(p, s, a, b);
-    const long long width = (b - a + p.splits - 1) / p.splits;
-    lo = a + part * width < b ? a + part * width : b;
-    hi = lo + width < b ? lo + width : b;
+// piece `part` of `splits` of rows [lo, hi)
+__device__ __forceinline__ void piece_of_pair(const PrefArgs& p, const PairRows& r, int part, long long& lo, long long& hi) {
+    const long long width = (r.hi - r.lo + p.splits - 1) / p.splits;
+    lo = r.lo + part * width < r.hi ? r.lo + part * width : r.hi;
+    hi = lo + width < r.hi ? lo + width : r.hi;
 }
-// w (logp - logp_ref) of one step; a step of weight 0: 0, whatever stands there
-__device__ __forceinline__ double step_gap(float lp, float ref, float w) {
-    return w == 0.f ? 0.0 : ((double)lp - (double)ref) * (double)w;
+// +- w (logp - logp_ref) of one step; a step of weight 0: 0, whatever stands there
+__device__ __forceinline__ double step_gap(float lp, float ref, float w, bool against) {
+    const double d = w == 0.f ? 0.0 : ((double)lp - (double)ref) * (double)w;
+    return against ? -d : d;
 }
 // a thread's share of rows [lo, hi): four steps a load (from any alignment), `id` of `n` threads
-__device__ __forceinline__ double span_sum(const PrefArgs& p, long long lo, long long hi, int id, int n) {
+__device__ __forceinline__ double span_sum(const PrefArgs& p, long long lo, long long hi, long long mid, int id, int n) {
     double v = 0.0;
     const long long full = lo + (hi - lo) / 4 * 4;
     for (long long t = lo + 4ll * id; t < full; t += 4ll * n) {
@@ -54,29 +63,26 @@ __device__ __forceinline__ double span_sum(const PrefArgs& p, long long lo, long
         load_pack<float, 4>(p.logp + t, a);
         if (p.logp_ref) load_pack<float, 4>(p.logp_ref + t, r);
         if (p.weight) load_pack<float, 4>(p.weight + t, w);
-        v += (step_gap(a[0], r[0], w[0]) + step_gap(a[1], r[1], w[1])) + (step_gap(a[2], r[2], w[2]) + step_gap(a[3], r[3], w[3]));
+        v += (step_gap(a[0], r[0], w[0], t >= mid) + step_gap(a[1], r[1], w[1], t + 1 >= mid)) +
+             (step_gap(a[2], r[2], w[2], t + 2 >= mid) + step_gap(a[3], r[3], w[3], t + 3 >= mid));
     }
     const long long t = full + id;
-    if (t < hi) v += step_gap(p.logp[t], p.logp_ref ? p.logp_ref[t] : 0.f, p.weight ? p.weight[t] : 1.f);
+    if (t < hi) v += step_gap(p.logp[t], p.logp_ref ? p.logp_ref[t] : 0.f, p.weight ? p.weight[t] : 1.f, t >= mid);
     return v;
 }
 // ... and its share of their gradients
 __device__ __forceinline__ float step_grad(double g, float w) { return w == 0.f ? 0.f : (float)(g * (double)w); }
-__device__ __forceinline__ void span_grad(const PrefArgs& p, long long lo, long long hi, int id, int n, double g) {
-    const float gf = (float)g;
+__device__ __forceinline__ void span_grad(const PrefArgs& p, long long lo, long long hi, long long mid, int id, int n, double g) {
     const long long full = lo + (hi - lo) / 4 * 4;
     for (long long t = lo + 4ll * id; t < full; t += 4ll * n) {
-        float d[4] = {gf, gf, gf, gf};
-        if (p.weight) {
-            float w[4];
-            load_pack<float, 4>(p.weight + t, w);
+        float d[4], w[4] = {1.f, 1.f, 1.f, 1.f};
+        if (p.weight) load_pack<float, 4>(p.weight + t, w);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) d[i] = step_grad(g, w[i]);
-        }
+        for (int i = 0; i < 4; ++i) d[i] = step_grad(t + i >= mid ? -g : g, w[i]);
         store_pack<float, 4>(p.dlogp + t, d);
     }
     const long long t = full + id;
-    if (t < hi) p.dlogp[t] = p.weight ? step_grad(g, p.weight[t]) : gf;
+    if (t < hi) p.dlogp[t] = step_grad(t >= mid ? -g : g, p.weight ? p.weight[t] : 1.f);
 }
 // rows outside every segment have no gradient
 __device__ __forceinline__ void outside_zero(const PrefArgs& p, long long id, long long n) {
@@ -118,13 +124,9 @@ __global__ __launch_bounds__(1024) void k_pref_small(PrefArgs p, float* __restri
     __shared__ double terms[PREF_SMALL_P * 3];
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
     for (int pair = wid; pair < p.P; pair += 16) {
-        long long a0, a1, b0, b1;
-        segment_of(p, 2 * pair, a0, a1);
-        segment_of(p, 2 * pair + 1, b0, b1);
-        const double delta = wave_sum(span_sum(p, a0, a1, lane, 64)) - wave_sum(span_sum(p, b0, b1, lane, 64));
-        const double g = pair_head(p, pair, delta, lane == 0, terms);
-        span_grad(p, a0, a1, lane, 64, g);
-        span_grad(p, b0, b1, lane, 64, -g);
+        const PairRows r = rows_of_pair(p, pair);
+        const double delta = wave_sum(span_sum(p, r.lo, r.hi, r.mid, lane, 64));
+        span_grad(p, r.lo, r.hi, r.mid, lane, 64, pair_head(p, pair, delta, lane == 0, terms));
     }
     outside_zero(p, threadIdx.x, 1024);
     __syncthreads();
@@ -138,51 +140,46 @@ __global__ __launch_bounds__(1024) void k_pref_small(PrefArgs p, float* __restri
 
 // Many pairs: a block per pair, sums and gradients in one launch.
 __global__ __launch_bounds__(256) void k_pref_pairs(PrefArgs p) {
-    __shared__ double red[8];
+    __shared__ double red[4];
     if (blockIdx.x >= (unsigned)p.P) {
         outside_zero(p, (long long)(blockIdx.x - p.P) * 256 + threadIdx.x, (long long)(gridDim.x - p.P) * 256);
         return;
     }
-    const int pair = blockIdx.x;
-    long long a0, a1, b0, b1;
-    segment_of(p, 2 * pair, a0, a1);
-    segment_of(p, 2 * pair + 1, b0, b1);
-    const double va = wave_sum(span_sum(p, a0, a1, threadIdx.x, 256)), vb = wave_sum(span_sum(p, b0, b1, threadIdx.x, 256));
-    if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6] = va; red[4 + (threadIdx.x >> 6)] = vb; }
+    const PairRows r = rows_of_pair(p, blockIdx.x);
+    const double v = wave_sum(span_sum(p, r.lo, r.hi, r.mid, threadIdx.x, 256));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    const double delta = (((red[0] + red[1]) + red[2]) + red[3]) - (((red[4] + red[5]) + red[6]) + red[7]);
-    const double g = pair_head(p, pair, delta, threadIdx.x == 0, p.terms);
-    span_grad(p, a0, a1, threadIdx.x, 256, g);
-    span_grad(p, b0, b1, threadIdx.x, 256, -g);
+    const double delta = ((red[0] + red[1]) + red[2]) + red[3];
+    span_grad(p, r.lo, r.hi, r.mid, threadIdx.x, 256, pair_head(p, blockIdx.x, delta, threadIdx.x == 0, p.terms));
 }
 
-// Few, long segments: a block per piece of one; its sum, then (every block joining its pair's pieces, in order) its gradients.
+// Few, long pairs: a block per piece of one; its sum, then (every block joining its pair's pieces, in order) its gradients.
 __global__ __launch_bounds__(256) void k_pref_sums(PrefArgs p) {
     __shared__ double red[4];
-    const int s = blockIdx.x / p.splits, part = blockIdx.x % p.splits;
+    const PairRows r = rows_of_pair(p, blockIdx.x / p.splits);
     long long lo, hi;
-    slice_of(p, s, part, lo, hi);
-    const double v = wave_sum(span_sum(p, lo, hi, threadIdx.x, 256));
+    piece_of_pair(p, r, blockIdx.x % p.splits, lo, hi);
+    const double v = wave_sum(span_sum(p, lo, hi, r.mid, threadIdx.x, 256));
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     if (threadIdx.x == 0) p.sums[blockIdx.x] = ((red[0] + red[1]) + red[2]) + red[3];
 }
 
 __global__ __launch_bounds__(256) void k_pref_grad(PrefArgs p) {
-    const unsigned blocks = 2u * p.P * p.splits;
+    const unsigned blocks = (unsigned)p.P * p.splits;
     if (blockIdx.x >= blocks) {
         outside_zero(p, (long long)(blockIdx.x - blocks) * 256 + threadIdx.x, (long long)(gridDim.x - blocks) * 256);
         return;
     }
-    const int s = blockIdx.x / p.splits, part = blockIdx.x % p.splits, pair = s >> 1;
-    const double* sums = p.sums + (size_t)pair * 2 * p.splits;
-    const int lane = threadIdx.x & 63;
+    const int pair = blockIdx.x / p.splits, part = blockIdx.x % p.splits, lane = threadIdx.x & 63;
+    const double* sums = p.sums + (size_t)pair * p.splits;
     double d = 0.0;
-    for (int i = lane; i < p.splits; i += 64) d += sums[i] - sums[p.splits + i];
-    const double g = pair_head(p, pair, wave_sum(d), threadIdx.x == 0 && part == 0 && (s & 1) == 0, p.terms);
+    for (int i = lane; i < p.splits; i += 64) d += sums[i];
+    const double g = pair_head(p, pair, wave_sum(d), threadIdx.x == 0 && part == 0, p.terms);
+    const PairRows r = rows_of_pair(p, pair);
     long long lo, hi;
-    slice_of(p, s, part, lo, hi);
-    span_grad(p, lo, hi, threadIdx.x, 256, (s & 1) ? -g : g);
+    piece_of_pair(p, r, part, lo, hi);
+    span_grad(p, lo, hi, r.mid, threadIdx.x, 256, g);
 }
 
 __global__ __launch_bounds__(FINISH_NT) void k_pref_finish(const double* __restrict__ terms, int P, float* __restrict__ loss3) {
@@ -508,12 +505,29 @@ __global__ __launch_bounds__(BAL_NT) void k_bal_stats(BalArgs p) {
             }
         }
     }
+    // one choice in the block: its groups in a wave add up first, a row of the merge is a wave (a block of 72 rows spent more time
+    // in the merge than a sixth of its work)
+    const bool single = p.AT == 1;
+    int merge = p.RR, my = at.rr;
+    bool writes = at.mine;
+    if (single) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            acc[e] = __uint_as_float(across_groups<G>(__float_as_uint(acc[e]), [](uint32_t a, uint32_t b) {
+                return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+            }));
+            cnt[e] = across_groups<G>(cnt[e], [](uint32_t a, uint32_t b) { return a + b; });
+        }
+        merge = blockDim.x / 64;
+        my = threadIdx.x >> 6;
+        writes = (threadIdx.x & 63) < G;
+    }
     __syncthreads();
-    if (at.mine) {
+    if (writes) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             if (ln.own(e)) {
-                sums[((size_t)at.rr * p.AT + at.al) * p.N + ln.at(e)] = acc[e];
+                sums[((size_t)my * p.AT + at.al) * p.N + ln.at(e)] = acc[e];
                 if (cnt[e]) atomicAdd(&cnts[at.al * p.N + ln.at(e)], cnt[e]);
             }
         }
@@ -523,7 +537,7 @@ __global__ __launch_bounds__(BAL_NT) void k_bal_stats(BalArgs p) {
     const int a0 = at.tile * p.AT, cols = (p.A - a0 < p.AT ? p.A - a0 : p.AT) * p.N;
     for (int i = threadIdx.x; i < cols; i += blockDim.x) {
         float s = 0.f;
-        for (int q = 0; q < p.RR; ++q) s += sums[(size_t)q * p.AT * p.N + i];
+        for (int q = 0; q < merge; ++q) s += sums[(size_t)q * p.AT * p.N + i];
         p.slab_p[(size_t)at.chunk * AN + (size_t)a0 * p.N + i] = s;
         p.slab_n[(size_t)at.chunk * AN + (size_t)a0 * p.N + i] = cnts[i];
     }
@@ -682,9 +696,9 @@ static void bal_shape(BalArgs& p) {
     p.RR = groups / p.AT;
     p.tiles = (p.A + p.AT - 1) / p.AT;
     // chunks of rows: two blocks a CU; four rows or more for a group of k_bal_stats (a chunk costs 8 A N bytes of slabs)
-    const long long most = ((long long)p.R + p.RR - 1) / p.RR, fill = (512 + p.tiles - 1) / p.tiles;
+    const long long most = ((long long)p.R + p.RR - 1) / p.RR, fill = (256 + p.tiles - 1) / p.tiles;
     p.chunks = (int)((most + 3) / 4 < fill ? (most + 3) / 4 : fill);
-    p.grad_chunks = (int)(most < 2 * fill ? most : 2 * fill);
+    p.grad_chunks = (int)(most < 4 * fill ? most : 4 * fill);
 }
 static size_t bal_terms(const BalArgs& p) { return ((size_t)p.A * p.N + BAL_COLS - 1) / BAL_COLS; }
 static size_t bal_bytes(const BalArgs& p) {
@@ -728,10 +742,9 @@ static void pick_bal(const BalArgs& p, hipStream_t st) {
 }
 
 static void pref_shape(PrefArgs& p) {
-    // pieces of a segment: about 4096 steps of the average one, and no more blocks than fill the chip a few times
-    const long long avg = p.T / (2ll * p.P);
-    long long s = (avg + 4095) / 4096;
-    const long long most = (8192 + 2ll * p.P - 1) / (2ll * p.P);
+    // pieces of a pair: about 8192 steps of the average one, and no more blocks than fill the chip a few times
+    long long s = (p.T / p.P + 8191) / 8192;
+    const long long most = (4096ll + p.P - 1) / p.P;
     if (s > most) s = most;
     p.splits = (int)(s < 1 ? 1 : s);
 }
@@ -747,7 +760,7 @@ size_t pfpn_preference_workspace_bytes(int P, long long T) {
     PrefArgs p = {};
     p.P = P; p.T = T;
     pref_shape(p);
-    return ((size_t)P * 3 + 2 * (size_t)P * p.splits) * sizeof(double);
+    return ((size_t)P * 3 + (size_t)P * p.splits) * sizeof(double);
 }
 
 int pfpn_preference_loss(const float* logp, const float* logp_ref, const float* weight, const int64_t* offsets, int P,
@@ -765,7 +778,7 @@ int pfpn_preference_loss(const float* logp, const float* logp_ref, const float* 
     p.terms = static_cast<double*>(workspace);
     p.sums = p.terms + (size_t)P * 3;
     hipStream_t st = (hipStream_t)stream;
-    const unsigned blocks = 2u * (unsigned)P * (unsigned)p.splits;
+    const unsigned blocks = (unsigned)P * (unsigned)p.splits;
     const unsigned outside = (unsigned)(T / 4096 + 1 < 64 ? T / 4096 + 1 : 64);
     if (P <= PREF_SMALL_P && T <= PREF_SMALL_T) {
         hipLaunchKernelGGL(k_pref_small, dim3(1), dim3(1024), 0, st, p, loss3);
