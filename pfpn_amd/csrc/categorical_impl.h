@@ -64,7 +64,12 @@ __device__ __forceinline__ double row_weight(const CatArgs& p, size_t b) {
 // rows, so the joint log-prob of a row and with it the upstream gradient are known inside the block: the loss takes ONE pass.
 // Phase 1: {l_k, m, s} of every segment into LDS; phase 2: the rows' log-probs and loss heads (64 bits), lanes_per_row lanes a
 // row; phase 3: the gradients from the exponentials that phase 1 left in registers (IT segments a group; IT = 0, rows too wide
-// for that: from the logits again, out of the caches).  Bound: HBM, one read of the logits and one write of the gradient.
+// for that: from the logits again, out of the caches).
+// Bound: HBM, one read of the logits and one write of the gradient.  8192 x 128 x 256 float32: 390 us = 5.5 TB/s (a 1-GiB copy on
+// the same card: 425 us); 4096 x 36 x 35: 14.4 us = 2.9 TB/s, one wave of blocks, latency and instructions (13 us of VALU issue).
+// What it measured on the way, 8192 x 128 x 256: reading the logits twice 933 us; holding 64 exponentials a thread, spilled around
+// the 64-bit head, 555 us; loads behind bounds branches (hipcc waits for each one) 511 us; clamped loads without a branch and half
+// of the exponentials parked in LDS 395 us.  Eight lanes x 5 for 35 particles, not 4 x 9: fewer waves, 14.1 against 16.2 us.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int MODE, int G, int E, int IT, int NT>
 __global__ __launch_bounds__(NT, E * IT > 32 ? 4 : 8) void k_cat_rows(CatArgs p) {
@@ -268,7 +273,11 @@ __global__ __launch_bounds__(NT, E * IT > 32 ? 4 : 8) void k_cat_rows(CatArgs p)
 // ---------------------------------------------------------------------------------------------------------------------
 // Long axes (N > 1024), enough rows to fill the chip: a block owns a segment and keeps ALL of it in registers (H wide loads a
 // thread, raw), so the logits are read once whatever their length: one pass finds {m, s}, the gradient is formed from the registers.
-// For A = 1 (a token row) the loss head sits in between, run by one wave.
+// For A = 1 (a token row) the loss head sits in between, run by one wave (three packs of eight wait in LDS meanwhile: its 64-bit
+// arithmetic would spill them).  1024 threads of at most 8 packs, two blocks a CU: one reads while the other writes.
+// Bound: HBM.  6001 x 50021 bfloat16, a fifth of the rows without weight: 235 us = 4.6 TB/s (two kernels that read the logits twice:
+// 337 us); gradient of 2047 x 32001 float16: 55 us = 4.8 TB/s (86 us).  It was bound by instructions (23 an element) until the
+// exponent became one fma, the maxima packed and the join of the waves a lane each: 60 -> 55 us, 253 -> 235 us.
 // ---------------------------------------------------------------------------------------------------------------------
 template <int NW>
 __device__ __forceinline__ void block_softmax(float m, float s, float* red, float& M, float& S) {

@@ -11,6 +11,8 @@ namespace pfpn {
 
 // ---------------------------------------------------------------------------------------------------------------------
 // The same loss on log-probs that come from elsewhere (the particle mixture's own density): one pass over [n] vectors.
+// 1000003 rows, weighted: 8.0 us + 2.3 us for the sum of the blocks (24 MB: 3.7 us at the cache's rate); 11.7 us with the
+// exponentials in 64 bits (80 double instructions a row).
 // ---------------------------------------------------------------------------------------------------------------------
 // Four rows a load, from any alignment.  One block (n <= 4096) finishes the sums itself.
 constexpr long long ROWS_SMALL = 4096;
@@ -68,7 +70,7 @@ __global__ __launch_bounds__(FINISH_NT) void k_policy_finish(const double* __res
 // host side
 // ---------------------------------------------------------------------------------------------------------------------
 int cat_splits(int B, int A, int N) {
-    // pieces of a long axis: blocks for the whole chip, pieces of at least 4096 logits
+    // pieces of a long axis: two blocks a CU, pieces of at least 4096 logits; one piece (the row held whole) from 512 segments on
     const long long segs = (long long)B * A;
     long long s = (512 + segs - 1) / segs;
     const long long most = ((long long)N + 4095) / 4096;

@@ -11,6 +11,9 @@ namespace pfpn {
 // with 2p + 1:  S_s = sum_t w_t (logp_t - logp_ref_t),  delta = S_2p - S_2p+1,  margin = beta delta,
 //   logistic:  -(1 - e) log sigma(margin) - e log sigma(-margin)      squared:  (delta - 1 / (2 beta))^2
 // mean over the pairs;  dlogp_t = +-(d loss / d delta) w_t.  Segment sums in 64 bits: thousands of terms, and their difference.
+// Bound: HBM / cache (12-16 bytes a step) for long segments; 1500 pairs of 3000017 steps: 15.3 us + 3.8 us for the sum of the pairs =
+// 3.1 TB/s, held back by what a block does once (bounds, 64-bit sums across lanes, the head): 128 threads a pair 18.5 us, 512 15.0 us,
+// 256 15.3 us with half the waves.  Two kernels, sums and gradients, took 38 us.  24 pairs: 5.3 us, one block, one launch (was 9 us).
 // =====================================================================================================================
 struct PrefArgs {
     const float* logp;
@@ -195,6 +198,10 @@ __global__ __launch_bounds__(FINISH_NT) void k_pref_finish(const double* __restr
 //   d l[b, a, n] = coef N / (A V) p_n (f_n - sum_m f_m p_m)         (f is a count: no gradient through it)
 // k_bal_stats leaves sums and counts of every chunk of rows as slabs, k_bal_reduce adds the slabs (64 bits, in order), k_bal_grad
 // writes the gradient.  A group of G lanes keeps ONE choice a while it walks rows: its sums, and f, stay in registers.
+// Bound: k_bal_stats instructions (the K-th largest), k_bal_grad HBM, k_bal_reduce latency.  262147 x 128 bfloat16, top 8, masked: 49 + 5 +
+// 31.5 us (two readings and a writing of 67 MB: 40 us); 4096 x 36 x 35 float32, top 1: 11.3 + 5.0 + 9.6 us (20 MB: 6.4 us, three launches).
+// Top 8 of 128 on the way: eight rounds of the group's maximum 117 us, rounds on sorted lists 74 us, joined lists of eight 66 us, keys that
+// hold the index (no ranking of equal logits afterwards) 57 us, 256 instead of 512 chunks of rows 49 us.
 // =====================================================================================================================
 struct BalArgs {
     const void* logits;
@@ -651,15 +658,15 @@ __global__ __launch_bounds__(BAL_NT) void k_bal_grad(BalArgs p) {
         }
         s = group_sum<G>(s);
         d = group_sum<G>(d);
-        const float inv = s == 0.f ? 0.f : 1.f / s, di = -d * inv * inv;
+        const float inv = s == 0.f ? 0.f : 1.f / s, dot = d * inv, di = -dot * inv;
         if (have && (row || !p.accumulate)) {               // (a masked row's gradient: zeros, or left alone)
             T* to = static_cast<T*>(p.dlogits) + b * p.ldd + off;
             T o[E];
             if (p.accumulate) ln.load(to, o);
-            // p_n (f_n - sum f p) with p = x / s, sum f p = d / s
+            // p_n (f_n - sum f p) with p = x / s, sum f p = d / s; 32-bit gradients form the difference, which cancels, first
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                float v = x[e] * __builtin_fmaf(f[e], inv, di);
+                float v = sizeof(T) == 4 ? (x[e] * inv) * (f[e] - dot) : x[e] * __builtin_fmaf(f[e], inv, di);
                 if (p.accumulate) v += to_f32(o[e]);
                 o[e] = from_f32<T>(row ? v : 0.f);
             }
