@@ -773,7 +773,10 @@ int run_cat(CatArgs p, void* ws, size_t ws_bytes, size_t* nparts, hipStream_t st
     const size_t segs = (size_t)p.B * p.A;
     const int S = cat_splits(p.B, p.A, p.N);
     if (segs * S > MAX_BLOCKS) return PFPN_ERR_ARG;
-    if (S == 1 && (p.A == 1 || MODE == CAT_BWD) && p.N <= 1024 * 16 * V) {
+    // A row held whole by one block takes one launch, pieces two or three.  One row of 8192 logits, float32, log-prob / gradient:
+    // 2.6 / 3.3 us held, 4.7 / 6.3 us in pieces; of 32768: 3.5 / 5.7 against 4.7 / 6.5; of 65536: 4.8 / 8.9 against 4.8 / 6.7, and
+    // 128 rows of 65536: 5.9 / 15.3 against 9.8 / 20.7 us.
+    if ((p.A == 1 || MODE == CAT_BWD) && p.N <= 1024 * 16 * V && (S == 1 || p.N <= 32768 || segs >= 128)) {
         if (p.N <= 256 * 4 * V) launch_held<T, MODE, 4, 256>(p, st);
         else if (p.N <= 512 * 4 * V) launch_held<T, MODE, 4, 512>(p, st);
         else if (p.N <= 1024 * 4 * V) launch_held<T, MODE, 4, 1024>(p, st);

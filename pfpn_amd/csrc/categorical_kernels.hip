@@ -70,7 +70,7 @@ __global__ __launch_bounds__(FINISH_NT) void k_policy_finish(const double* __res
 // host side
 // ---------------------------------------------------------------------------------------------------------------------
 int cat_splits(int B, int A, int N) {
-    // pieces of a long axis: two blocks a CU, pieces of at least 4096 logits; one piece (the row held whole) from 512 segments on
+    // pieces of a long axis: two blocks a CU, pieces of at least 4096 logits; one piece from 512 segments on
     const long long segs = (long long)B * A;
     long long s = (512 + segs - 1) / segs;
     const long long most = ((long long)N + 4095) / 4096;

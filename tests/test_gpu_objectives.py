@@ -12,6 +12,7 @@ TYPES = [torch.float32, torch.bfloat16, torch.float16]
 SHAPES = [(1, 1, 1), (1, 1, 2), (3, 2, 1), (1, 36, 35), (33, 36, 35), (257, 5, 8), (64, 3, 9), (33, 2, 17), (20, 7, 25), (19, 7, 33),
           (5, 130, 41), (7, 13, 64), (5, 3, 65), (5, 3, 96), (9, 4, 97), (9, 4, 128), (6, 2, 129), (6, 2, 192), (5, 3, 193), (5, 128, 256),
           (4, 2, 257), (4, 2, 512), (3, 2, 513), (3, 2, 1024), (2, 3, 1025), (5, 1, 4097), (1, 3, 8191), (3, 1, 50021), (1, 1, 128000),
+          (1, 1, 8191), (2, 1, 32768), (2, 2, 32769), (2, 1, 65536), (128, 1, 65536), (130, 1, 65541),
           (700, 1, 1500), (2, 4096, 3), (1025, 1, 37), (4, 36, 35), (9, 7, 1100), (2, 600, 1030), (3, 700, 300), (2100, 1, 300)]
 
 
