@@ -28,7 +28,7 @@ struct CatArgs {
 };
 
 __device__ __forceinline__ void write_loss4(const double* sums, double kl_coef, float* loss4) {
-    loss4[0] = (float)(sums[0] + kl_coef * sums[1]);
+    loss4[0] = (float)(kl_coef != 0.0 ? sums[0] + kl_coef * sums[1] : sums[0]);
     loss4[1] = (float)sums[0];
     loss4[2] = (float)sums[1];
     loss4[3] = (float)sums[2];
@@ -773,6 +773,9 @@ int run_cat(CatArgs p, void* ws, size_t ws_bytes, size_t* nparts, hipStream_t st
     const size_t segs = (size_t)p.B * p.A;
     const int S = cat_splits(p.B, p.A, p.N);
     if (segs * S > MAX_BLOCKS) return PFPN_ERR_ARG;
+    const size_t pieces = segs * S;
+    if (!ws || ws_bytes < parts + pieces * 2 * sizeof(float) + (MODE == CAT_PPO ? (size_t)p.B * sizeof(float) : 0))
+        return PFPN_ERR_WORKSPACE;
     // A row held whole by one block takes one launch, pieces two or three.  One row of 8192 logits, float32, log-prob / gradient:
     // 2.6 / 3.3 us held, 4.7 / 6.3 us in pieces; of 32768: 3.5 / 5.7 against 4.7 / 6.5; of 65536: 4.8 / 8.9 against 4.8 / 6.7, and
     // 128 rows of 65536: 5.9 / 15.3 against 9.8 / 20.7 us.
@@ -785,9 +788,6 @@ int run_cat(CatArgs p, void* ws, size_t ws_bytes, size_t* nparts, hipStream_t st
         PFPN_CHECK_LAUNCH();
         return PFPN_OK;
     }
-    const size_t pieces = segs * S;
-    if (!ws || ws_bytes < parts + pieces * 2 * sizeof(float) + (MODE == CAT_PPO ? (size_t)p.B * sizeof(float) : 0))
-        return PFPN_ERR_WORKSPACE;
     float* stats = reinterpret_cast<float*>(static_cast<char*>(ws) + parts);
     hipLaunchKernelGGL((k_cat_long_stats<T>), dim3((unsigned)pieces), dim3(LONG_NT), 0, st, p, S, MODE, stats);
     constexpr int ROWS = MODE == CAT_PPO ? CAT_PPO : CAT_FWD;

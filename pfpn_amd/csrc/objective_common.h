@@ -289,7 +289,7 @@ __device__ __forceinline__ double policy_head(double logp, const HeadRow& row, c
     if (h.logp_ref) {
         float em1;
         kl = kl_sample((float)((double)row.logp_ref - logp), em1);
-        g -= h.kl_coef * (double)em1;
+        if (h.kl_coef != 0.0) g -= h.kl_coef * (double)em1;        // (a term that is only reported may be infinite)
     }
     t.policy = row.w * (clipped ? -(double)held : -(double)sur);
     t.kl = row.w * (double)kl;

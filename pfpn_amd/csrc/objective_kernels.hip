@@ -104,7 +104,7 @@ __device__ __forceinline__ double pair_head(const PrefArgs& p, int pair, double 
         const float z = expf(-am), l = log1pf(z), near = 1.f / (1.f + z), far = z * near;
         const float good = m >= 0 ? near : far, bad = m >= 0 ? far : near;
         const float sp_neg = l + (m < 0 ? am : 0.f), sp_pos = l + (m > 0 ? am : 0.f);
-        loss = (1.f - e) * sp_neg + e * sp_pos;
+        loss = (1.f - e) * sp_neg + (e > 0.f ? e * sp_pos : 0.f);      // (an infinite margin: 0, not 0 * inf)
         slope = p.beta * (double)(e * good - (1.f - e) * bad);
         if (m != m) { loss = m; slope = m; }
     } else {

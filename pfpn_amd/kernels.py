@@ -578,8 +578,8 @@ def _logit_rows(t, name="logits"):
     ld = stride[0] if B > 1 else A * N
     if not dense or ld < A * N:
         raise ValueError("%s: only the rows may be strided (shape %s, strides %s)" % (name, tuple(shape), stride))
-    if A > 4096 or N > 1 << 30:
-        raise ValueError("%s has shape %s: at most 4096 choices of 2^30 categories" % (name, tuple(shape)))
+    if A > 4096 or N > 1 << 30 or B >= 1 << 31:
+        raise ValueError("%s has shape %s: less than 2^31 rows of at most 4096 choices of 2^30 categories" % (name, tuple(shape)))
     return t.data_ptr(), _LOGIT_TYPES[t.dtype], ld, B, A, N
 
 
@@ -715,7 +715,7 @@ def policy_kl_loss(logp, logp_old, adv, logp_ref=None, weight=None, stats=None, 
     dlogp = torch.empty(n, dtype=torch.float32, device=dev) if dlogp is None else dlogp
     loss4 = torch.empty(4, dtype=torch.float32, device=dev) if loss4 is None else loss4
     pd, p4 = _rows(dlogp, n, dev, "dlogp"), _rows(loss4, 4, dev, "loss4")
-    if pd == pl and n:
+    if abs(pd - pl) < 4 * n:
         raise ValueError("dlogp overlaps logp")
     if n == 0:
         loss4.zero_()
@@ -731,6 +731,18 @@ def policy_kl_loss(logp, logp_old, adv, logp_ref=None, weight=None, stats=None, 
 _PREFERENCE_KINDS = {"logistic": 0, "squared": 1}
 
 
+def pair_count(offsets, device):
+    """P of the bounds [2P+1] of P pairs of segments (preference_loss), checked for type, place and number"""
+    if not (isinstance(offsets, torch.Tensor) and offsets.is_cuda and offsets.dtype == torch.int64 and offsets.is_contiguous() and
+            offsets.dim() == 1 and offsets.device == device):
+        raise ValueError("offsets must be a contiguous int64 [2P + 1] tensor on the log-probs' device")
+    if offsets.shape[0] < 3 or offsets.shape[0] % 2 == 0:
+        raise ValueError("offsets holds %d bounds: an odd number, two segments for each pair, is needed" % offsets.shape[0])
+    if offsets.shape[0] // 2 > 1 << 22:
+        raise ValueError("at most 2^22 pairs")
+    return offsets.shape[0] // 2
+
+
 def preference_loss(logp, offsets, logp_ref=None, weight=None, beta=0.1, label_smoothing=0.0, kind="logistic"):
     """Loss over pairs of compared segments of per-step log-probs [T].  offsets [2P+1] int64 (device, ascending): segment s =
     rows offsets[s] .. offsets[s+1] - 1, pair p prefers segment 2p to segment 2p + 1.  `logp_ref` [T]: the same steps under a
@@ -740,18 +752,11 @@ def preference_loss(logp, offsets, logp_ref=None, weight=None, beta=0.1, label_s
         raise ValueError("logp must be a [T] tensor")
     T, dev = logp.shape[0], logp.device
     pl = _rows(logp, T, dev, "logp")
-    if not (isinstance(offsets, torch.Tensor) and offsets.is_cuda and offsets.dtype == torch.int64 and offsets.is_contiguous() and
-            offsets.dim() == 1 and offsets.device == dev):
-        raise ValueError("offsets must be a contiguous int64 [2P + 1] tensor on the log-probs' device")
-    if offsets.shape[0] < 3 or offsets.shape[0] % 2 == 0:
-        raise ValueError("offsets holds %d bounds: an odd number, two segments for each pair, is needed" % offsets.shape[0])
-    P = offsets.shape[0] // 2
-    if P > 1 << 22:
-        raise ValueError("at most 2^22 pairs")
+    P = pair_count(offsets, dev)
     if kind not in _PREFERENCE_KINDS:
         raise ValueError("kind is one of %s" % sorted(_PREFERENCE_KINDS))
-    if not float(beta) > 0.0 or not 0.0 <= float(label_smoothing) <= 0.5:
-        raise ValueError("beta > 0 and label_smoothing in [0, 0.5] are needed")
+    if not 0.0 < float(beta) < float("inf") or not 0.0 <= float(label_smoothing) <= 0.5:
+        raise ValueError("a finite beta > 0 and label_smoothing in [0, 0.5] are needed")
     if label_smoothing and kind != "logistic":
         raise ValueError("label_smoothing belongs to the logistic loss")
     pr = _rows(logp_ref, T, dev, "logp_ref") if logp_ref is not None else None

@@ -321,6 +321,39 @@ def test_preference_gradient_against_differences(dev):
     assert float((d.double().cpu() - num).abs().max()) < 1e-6       # (the slope, under 0.25, is off by 16 steps of 2^-24 at most)
 
 
+def test_reported_kl_of_an_impossible_choice_stays_out_of_the_loss(dev):
+    """kl_coef = 0 with a reference: the KL term is reported (infinite here), loss and gradient are those without it"""
+    from pfpn_amd import kernels
+    for B, A, N in ((6, 3, 7), (3, 1, 5000), (2, 1, 70001)):
+        x, k, g = make_logits(dev, B, A, N, torch.float32, seed=9)
+        x, k = x.contiguous(), k.clamp(min=1)
+        x[0].scatter_(-1, k[0].unsqueeze(-1), -math.inf)
+        old, adv, ref = torch.full((B,), -5.0, device=dev), torch.randn(B, device=dev, generator=g), torch.full((B,), -5.0, device=dev)
+        want = kernels.categorical_ppo_fwd_bwd(x, k, old, adv)
+        got = kernels.categorical_ppo_fwd_bwd(x, k, old, adv, logp_ref=ref)
+        assert got["loss4"][2] == math.inf and torch.isfinite(got["loss4"][:2]).all()
+        assert torch.equal(got["dlogits"], want["dlogits"]) and torch.equal(got["loss4"][[0, 1, 3]], want["loss4"][[0, 1, 3]])
+    logp = torch.tensor([-math.inf, -3.0], device=dev)
+    d, l4 = kernels.policy_kl_loss(logp, logp.clamp(min=-4), torch.ones(2, device=dev), logp_ref=torch.zeros(2, device=dev))
+    assert torch.isfinite(d).all() and l4[2] == math.inf and torch.isfinite(l4[:2]).all()
+
+
+@pytest.mark.parametrize("T,lengths", [(6, [3, 3]), (60000, [30000, 30000]), (40000, [20, 20] * 1000)])
+def test_preference_for_an_impossible_segment(dev, T, lengths):
+    """an infinite margin: won pairs have no loss and no gradient, lost ones an infinite loss and the steepest gradient"""
+    from pfpn_amd import kernels
+    P, offsets = len(lengths) // 2, torch.tensor([0] + lengths, device=dev).cumsum(0)
+    for at, loss, slope in ((lengths[0], 0.0, 0.0), (0, math.inf, 0.1)):       # first step of the pair's second / first segment
+        logp = torch.full((T,), -1.0, device=dev)
+        starts = offsets[:-1].view(P, 2)[:, 0] + at
+        logp[starts] = -math.inf
+        d, m, l3 = kernels.preference_loss(logp, offsets, beta=0.1)
+        assert bool(torch.isinf(m).all()) and l3[0] == loss
+        want = torch.full((T,), slope / P, device=dev)
+        sign = torch.repeat_interleave(torch.tensor([-1.0, 1.0] * P, device=dev), torch.tensor(lengths, device=dev))
+        close(d, want * sign, 4 * U * want.abs())                   # (products and a quotient of 32 bits)
+
+
 def test_preference_bad_bounds_stay_inside(dev):
     """bounds outside [0, T] are clamped, descending ones make an empty segment: nothing outside the vectors is touched"""
     from pfpn_amd import kernels
@@ -428,7 +461,11 @@ def test_refusals_on_the_device(dev):
         with pytest.raises(ValueError):
             kernels.preference_loss(b, bad)
     off = torch.tensor([0, 2, 4], device=dev)
-    for kw in ({"beta": 0.0}, {"beta": -1.0}, {"kind": "hinge"}, {"label_smoothing": 0.7}, {"kind": "squared", "label_smoothing": 0.1}):
+    with pytest.raises(ValueError, match="overlap"):
+        kernels.policy_kl_loss(wide.view(-1)[:20], *[torch.zeros(20, device=dev)] * 2, dlogp=wide.view(-1)[10:30])
+    with pytest.raises(ValueError, match="2\\^31"):        # (the C entry takes the number of rows in 32 bits)
+        kernels.categorical_logprob_fwd(torch.empty((1 << 31) + 8, 1, dtype=torch.float16, device=dev), k)
+    for kw in ({"beta": 0.0}, {"beta": math.inf}, {"beta": -1.0}, {"kind": "hinge"}, {"label_smoothing": 0.7}, {"kind": "squared", "label_smoothing": 0.1}):
         with pytest.raises(ValueError):
             kernels.preference_loss(b, off, **kw)
     for kw in ({"topk": 0}, {"topk": 6}, {"mask": torch.ones(3, dtype=torch.bool, device=dev)}, {"mask": torch.ones(4, device=dev)},
