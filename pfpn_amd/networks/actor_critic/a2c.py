@@ -105,7 +105,7 @@ class ParticleFilteringA2CNetwork(A2CNetwork):
         self.preference_beta, self.preference_smoothing = float(preference_beta), float(preference_smoothing)
         if balance_beta and self.particles > 1024:
             raise ValueError("balance_beta: at most 1024 particles")
-        if not self.preference_beta > 0.0 or not 0.0 <= self.preference_smoothing <= 0.5:
+        if not 0.0 < self.preference_beta < float("inf") or not 0.0 <= self.preference_smoothing <= 0.5:
             raise ValueError("preference_beta > 0 and preference_smoothing in [0, 0.5] are needed")
         self._reference = None
 
@@ -272,6 +272,10 @@ class ParticleFilteringA2CNetwork(A2CNetwork):
         optional (discounts, a mask).  Log ratios are taken to the reference where set_reference() was called.  The critic
         gets no gradient.  Gradients land in self.store.grad; returns loss3 (device): {loss, share of pairs won, mean margin}."""
         B = state.shape[0]
+        kernels.pair_count(offsets, state.device)           # (refused before the normaliser has seen the states)
+        if action.shape[0] != B or (weight is not None and weight.shape != (B,)):
+            raise ValueError("%d states, actions %s, weight %s" % (B, tuple(action.shape),
+                                                                   None if weight is None else tuple(weight.shape)))
         self._ensure_buffers(B)
         deferred = self._deferred_jobs(B)
         x = self.prologue(state, deferred=deferred)
@@ -309,6 +313,8 @@ class ParticleFilteringA2CNetwork(A2CNetwork):
         if st.shape[0] == 0 or st.shape[0] != ac.shape[0]:
             raise ValueError("train_preference: %d states, %d actions" % (st.shape[0], ac.shape[0]))
         offs = torch.as_tensor(offsets, dtype=torch.int64)
+        if offs.dim() != 1 or offs.shape[0] < 3:
+            raise ValueError("train_preference: offsets are the 2P + 1 bounds of the segments of P pairs")
         if not offs.is_cuda and (int(offs[0]) < 0 or int(offs[-1]) > st.shape[0] or bool((offs[1:] < offs[:-1]).any())):
             raise ValueError("train_preference: offsets ascend within [0, %d]" % st.shape[0])
         offs = offs.to(self.device).contiguous()

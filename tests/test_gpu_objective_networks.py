@@ -197,6 +197,22 @@ def test_train_preference_api(dev):
         net.train_preference(None, opt, [], b["state"], b["action"][:20], [0, 10, 20])
 
 
+def test_refused_preference_steps_change_nothing(dev, monkeypatch):
+    """bounds, weights or actions that do not fit are refused before the step begins: the normaliser has not seen the states"""
+    from pfpn_amd.models import SyncReplicasApplier
+    net = make(dev)
+    opt = SyncReplicasApplier(net, [{"names": None, "lr": 1e-3}], norm_clip=1.0, world_size=1)
+    b = batch(50, 1)
+    monkeypatch.setattr(net, "prologue", lambda *a, **k: pytest.fail("the step began"))
+    for offsets, weight in (([], None), ([0], None), ([0, 10], None), ([0, 10, 20, 30], None), ([[0, 10, 20]], None),
+                            ([0, 10, 20], np.ones(49, np.float32))):
+        with pytest.raises(ValueError):
+            net.train_preference(None, opt, [], b["state"], b["action"], offsets, weight)
+    with pytest.raises(ValueError):
+        net.compute_preference_gradients(torch.from_numpy(b["state"]).to(dev), torch.from_numpy(b["action"]).to(dev)[:49],
+                                         torch.tensor([0, 10, 20], device=dev))
+
+
 @pytest.mark.parametrize("round_rows", [0, 512])
 def test_captured_steps_equal_eager_ones(dev, monkeypatch, round_rows):
     """minibatch steps with the KL term and the balance loss: the replayed steps leave the eager steps' bits, the counts of the

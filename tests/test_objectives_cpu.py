@@ -1,4 +1,6 @@
 """CPU: what the policy objectives refuse, through the package and through the C ABI (before any launch)."""
+import math
+
 import pytest
 import torch
 
@@ -99,7 +101,7 @@ def test_network_options():
     from pfpn_amd import networks
     base = dict(trainable=True, state_shape=[5], action_shape=[2], action_lower_bound=[-1, -1], action_upper_bound=[1, 1],
                 common_net_shape=[], critic_net_shape=[8], actor_net_shape=[8])
-    for bad in (dict(kl_coef=-0.1), dict(preference_beta=0.0), dict(preference_smoothing=0.6), dict(balance_beta=0.1, particles=1025)):
+    for bad in (dict(kl_coef=-0.1), dict(preference_beta=0.0), dict(preference_beta=math.inf), dict(preference_smoothing=0.6), dict(balance_beta=0.1, particles=1025)):
         with pytest.raises(ValueError):
             networks.ParticleFilteringClipPPONetwork(**base, **bad)
     with pytest.raises(NotImplementedError):
