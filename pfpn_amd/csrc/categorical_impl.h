@@ -221,7 +221,7 @@ __global__ __launch_bounds__(NT, E * IT > 32 ? 4 : 8) void k_cat_rows(CatArgs p)
                 if (v.k >= 0) lp += v.s == 0.f ? (double)-INFINITY : (double)v.xk - (double)v.m - log((double)v.s);
             }
         }
-        for (int o = 1; o < LP; o <<= 1) lp += __shfl_xor(lp, o, 64);
+        lp = LP == 1 ? lp : LP == 4 ? group_sum<4>(lp) : LP == 16 ? group_sum<16>(lp) : group_sum<64>(lp);
         if (tid % LP == 0 && my_row < rows) {
             p.logp[row0 + my_row] = (float)lp;
             if (MODE == CAT_PPO) {
@@ -260,7 +260,7 @@ __global__ __launch_bounds__(NT, E * IT > 32 ? 4 : 8) void k_cat_rows(CatArgs p)
     if (wid < 3) {
         double t = 0.0;
         for (int r = lane; r < rows; r += 64) t += terms[r * 3 + wid];
-        t = wave_sum(t);
+        t = group_sum<64>(t);
         if (lane == 0 && !p.loss4) p.part[(size_t)blockIdx.x * 3 + wid] = t;
         if (lane == 0 && p.loss4) terms[(rows - 1) * 3 + wid] = t;      // (the last row's terms have been added)
     }
@@ -271,7 +271,7 @@ __global__ __launch_bounds__(NT, E * IT > 32 ? 4 : 8) void k_cat_rows(CatArgs p)
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Long axes (N > 1024), enough rows to fill the chip: a block owns a segment and keeps ALL of it in registers (H wide loads a
+// Long axes (N > 1024), rows that one block can hold (few very long ones: in pieces, below): a block owns a segment and keeps ALL of it in registers (H wide loads a
 // thread, raw), so the logits are read once whatever their length: one pass finds {m, s}, the gradient is formed from the registers.
 // For A = 1 (a token row) the loss head sits in between, run by one wave (three packs of eight wait in LDS meanwhile: its 64-bit
 // arithmetic would spill them).  1024 threads of at most 8 packs, two blocks a CU: one reads while the other writes.
@@ -502,7 +502,7 @@ __global__ __launch_bounds__(NT, H > 8 ? 4 : 8) void k_cat_long_held(CatArgs p) 
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Long axes, few rows, several long choices in a row, or an axis beyond the registers: a block owns one of `splits` pieces of a
-// segment.  k_cat_long_stats leaves {m, s} of every piece, k_cat_long_logp joins them to log-probs, k_cat_long_grad joins them
+// segment.  k_cat_long_stats leaves {m, s} of every piece, k_cat_long_rows joins them to log-probs, k_cat_long_grad joins them
 // (every block its own row's, in the same order: the same bits) and writes its piece of the gradient.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int LONG_NT = 256;

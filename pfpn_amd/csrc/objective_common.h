@@ -150,6 +150,36 @@ __device__ __forceinline__ float group_sum(float v) {
         return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
     }));
 }
+// (64 bits: both halves move, where a shuffle through LDS takes six round trips)
+__device__ __forceinline__ double halves(uint32_t lo, uint32_t hi) {
+    return __longlong_as_double((long long)((unsigned long long)hi << 32 | lo));
+}
+template <int CTRL>
+__device__ __forceinline__ double add_moved(double v) {
+    const unsigned long long b = (unsigned long long)__double_as_longlong(v);
+    const uint32_t lo = lane_move<CTRL>((uint32_t)b), hi = lane_move<CTRL>((uint32_t)(b >> 32));
+    return v + halves(lo, hi);
+}
+template <int G>
+__device__ __forceinline__ double group_sum(double v) {
+    if (G > 1) v = add_moved<0xB1>(v);
+    if (G > 2) v = add_moved<0x4E>(v);
+    if (G > 4) v = add_moved<0x141>(v);
+    if (G > 8) v = add_moved<0x140>(v);
+    if (G > 16) {
+        const unsigned long long b = (unsigned long long)__double_as_longlong(v);
+        const auto l = __builtin_amdgcn_permlane16_swap((uint32_t)b, (uint32_t)b, false, false);
+        const auto h = __builtin_amdgcn_permlane16_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+        v = halves(l[0], h[0]) + halves(l[1], h[1]);
+    }
+    if (G > 32) {
+        const unsigned long long b = (unsigned long long)__double_as_longlong(v);
+        const auto l = __builtin_amdgcn_permlane32_swap((uint32_t)b, (uint32_t)b, false, false);
+        const auto h = __builtin_amdgcn_permlane32_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+        v = halves(l[0], h[0]) + halves(l[1], h[1]);
+    }
+    return v;
+}
 template <int G>
 __device__ __forceinline__ uint32_t group_min(uint32_t v) {
     return group_reduce<G>(v, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
@@ -300,7 +330,7 @@ __device__ __forceinline__ double policy_head(double logp, const HeadRow& row, c
 // per-block sums {policy, kl, clipped} -> part[3]; `red` needs 3 * 16 doubles of LDS.  Fixed order.
 __device__ __forceinline__ void block_terms(const HeadTerms& t, double* red, double* part) {
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, nw = (blockDim.x + 63) >> 6;
-    const double a = wave_sum(t.policy), b = wave_sum(t.kl), c = wave_sum(t.clipped);
+    const double a = group_sum<64>(t.policy), b = group_sum<64>(t.kl), c = group_sum<64>(t.clipped);
     __syncthreads();
     if (lane == 0) { red[wid * 3] = a; red[wid * 3 + 1] = b; red[wid * 3 + 2] = c; }
     __syncthreads();
@@ -328,7 +358,7 @@ __device__ __forceinline__ void sum_terms(const double* __restrict__ part, size_
 #pragma unroll
         for (int k = 0; k < DEEP; ++k) s += i + LANES * k < n ? t[k] : 0.0;
     }
-    s = wave_sum(s);
+    s = group_sum<64>(s);
     if (lane == 0) red[wid] = s;
     __syncthreads();
     if (threadIdx.x < 3) {

@@ -94,7 +94,7 @@ __device__ __forceinline__ void outside_zero(const PrefArgs& p, long long id, lo
     for (long long t = (last < 0 ? 0 : last) + id; t < p.T; t += n) p.dlogp[t] = 0.f;
 }
 
-// loss of one pair -> d loss / d delta (of the mean); fills terms and margin when `write`
+// loss of one pair -> d loss / d delta (of the mean); fills its terms[3] and margin when `write`
 __device__ __forceinline__ double pair_head(const PrefArgs& p, int pair, double delta, bool write, double* terms) {
     const double m = p.beta * delta;
     double loss, slope;
@@ -114,34 +114,37 @@ __device__ __forceinline__ double pair_head(const PrefArgs& p, int pair, double 
     }
     if (write) {
         p.margin[pair] = (float)m;
-        terms[(size_t)pair * 3] = loss;
-        terms[(size_t)pair * 3 + 1] = m > 0 ? 1.0 : 0.0;
-        terms[(size_t)pair * 3 + 2] = m;
+        terms[0] = loss;
+        terms[1] = m > 0 ? 1.0 : 0.0;
+        terms[2] = m;
     }
     return slope / (double)p.P;
 }
 
 // Few steps: ONE block, a wave per pair in turn (a launch costs more than the work).
-constexpr int PREF_SMALL_P = 128, PREF_SMALL_T = 16384;
+// (PREF_SHORT: up to so many steps a pair, many pairs go by lanes, not by blocks.  20000 pairs of 100: 44 us by blocks, 25 us by waves,
+// 12 us by 16 lanes with the blocks' terms summed; 3000 of 1000: 13.9 / 13.0 us; but 400 of 1000: 7.3 us by blocks, 8.5 us by waves,
+// which are too few to fill the chip)
+constexpr int PREF_SHORT = 1024, PREF_SMALL_P = 128, PREF_SMALL_T = 16384;
 __global__ __launch_bounds__(1024) void k_pref_small(PrefArgs p, float* __restrict__ loss3) {
     __shared__ double terms[PREF_SMALL_P * 3];
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
     for (int pair = wid; pair < p.P; pair += 16) {
         const PairRows r = rows_of_pair(p, pair);
-        const double delta = wave_sum(span_sum(p, r.lo, r.hi, r.mid, lane, 64));
-        span_grad(p, r.lo, r.hi, r.mid, lane, 64, pair_head(p, pair, delta, lane == 0, terms));
+        const double delta = group_sum<64>(span_sum(p, r.lo, r.hi, r.mid, lane, 64));
+        span_grad(p, r.lo, r.hi, r.mid, lane, 64, pair_head(p, pair, delta, lane == 0, terms + pair * 3));
     }
     outside_zero(p, threadIdx.x, 1024);
     __syncthreads();
     if (wid < 3) {
         double t = 0.0;
         for (int i = lane; i < p.P; i += 64) t += terms[i * 3 + wid];
-        t = wave_sum(t);
+        t = group_sum<64>(t);
         if (lane == 0) loss3[wid] = (float)(t / (double)p.P);
     }
 }
 
-// Many pairs: a block per pair, sums and gradients in one launch.
+// Pairs that fill a block: a block per pair, sums and gradients in one launch.
 __global__ __launch_bounds__(256) void k_pref_pairs(PrefArgs p) {
     __shared__ double red[4];
     if (blockIdx.x >= (unsigned)p.P) {
@@ -149,11 +152,108 @@ __global__ __launch_bounds__(256) void k_pref_pairs(PrefArgs p) {
         return;
     }
     const PairRows r = rows_of_pair(p, blockIdx.x);
-    const double v = wave_sum(span_sum(p, r.lo, r.hi, r.mid, threadIdx.x, 256));
+    constexpr int H = 4;
+    if (r.hi - r.lo >= 4 * 256 && r.hi - r.lo < 4 * 256 * H) {
+        // all of the pair's steps in flight at once (packs past the end: the last one again), the weights held for the gradients:
+        // 3000 pairs of 4095 steps 41 -> 33 us; pairs of 1000, which would read the last pack three times, 9.5 -> 11.1 us
+        const int steps = (int)(r.hi - r.lo), mid = (int)(r.mid - r.lo), packs = steps / 4, tail = packs * 4 + (int)threadIdx.x;
+        const float *lp = p.logp + r.lo, *ref = p.logp_ref + r.lo, *wt = p.weight + r.lo;
+        float a[H][4], q[H][4] = {}, w[H][4], at = 0.f, qt = 0.f, wl = 1.f;
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[h][i] = 1.f;
+        int where[H];
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            const int i = h * 256 + (int)threadIdx.x;
+            where[h] = 4 * (i < packs ? i : packs - 1);
+        }
+#pragma unroll
+        for (int h = 0; h < H; ++h) load_pack<float, 4>(lp + where[h], a[h]);
+        if (p.logp_ref) {
+#pragma unroll
+            for (int h = 0; h < H; ++h) load_pack<float, 4>(ref + where[h], q[h]);
+        }
+        if (p.weight) {
+#pragma unroll
+            for (int h = 0; h < H; ++h) load_pack<float, 4>(wt + where[h], w[h]);
+        }
+        if (tail < steps) {
+            at = lp[tail];
+            if (p.logp_ref) qt = ref[tail];
+            if (p.weight) wl = wt[tail];
+        }
+        double v = 0.0;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            const int t = where[h];
+            const double part = (step_gap(a[h][0], q[h][0], w[h][0], t >= mid) + step_gap(a[h][1], q[h][1], w[h][1], t + 1 >= mid)) +
+                                (step_gap(a[h][2], q[h][2], w[h][2], t + 2 >= mid) + step_gap(a[h][3], q[h][3], w[h][3], t + 3 >= mid));
+            v += h * 256 + (int)threadIdx.x < packs ? part : 0.0;
+        }
+        if (tail < steps) v += step_gap(at, qt, wl, tail >= mid);
+        v = group_sum<64>(v);
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        const double delta = ((red[0] + red[1]) + red[2]) + red[3];
+        const double g = pair_head(p, blockIdx.x, delta, threadIdx.x == 0, p.terms + (size_t)blockIdx.x * 3);
+        float* d = p.dlogp + r.lo;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            if (h * 256 + (int)threadIdx.x < packs) {
+                float o[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = step_grad(where[h] + i >= mid ? -g : g, w[h][i]);
+                store_pack<float, 4>(d + where[h], o);
+            }
+        }
+        if (tail < steps) d[tail] = step_grad(tail >= mid ? -g : g, wl);
+        return;
+    }
+    const double v = group_sum<64>(span_sum(p, r.lo, r.hi, r.mid, threadIdx.x, 256));
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     const double delta = ((red[0] + red[1]) + red[2]) + red[3];
-    span_grad(p, r.lo, r.hi, r.mid, threadIdx.x, 256, pair_head(p, blockIdx.x, delta, threadIdx.x == 0, p.terms));
+    span_grad(p, r.lo, r.hi, r.mid, threadIdx.x, 256, pair_head(p, blockIdx.x, delta, threadIdx.x == 0, p.terms + (size_t)blockIdx.x * 3));
+}
+
+// Many short pairs: G lanes a pair, no barrier between sums and gradients; a block leaves the sum of its pairs' terms (fixed order).
+template <int G>
+__global__ __launch_bounds__(256) void k_pref_groups(PrefArgs p, int blocks) {
+    constexpr int PER = 256 / G;
+    __shared__ double red[3 * PER];
+    if (blockIdx.x >= (unsigned)blocks) {
+        outside_zero(p, (long long)(blockIdx.x - blocks) * 256 + threadIdx.x, (long long)(gridDim.x - blocks) * 256);
+        return;
+    }
+    const int lane = threadIdx.x % G;
+    double t[3] = {0.0, 0.0, 0.0};
+    for (int first = blockIdx.x * PER; first < p.P; first += blocks * PER) {
+        const int pair = first + (int)threadIdx.x / G;
+        const bool on = pair < p.P;
+        const PairRows r = rows_of_pair(p, on ? pair : p.P - 1);
+        double delta = on ? span_sum(p, r.lo, r.hi, r.mid, lane, G) : 0.0;
+        delta = group_sum<G>(delta);
+        if (on) {
+            double own[3];
+            const double g = pair_head(p, pair, delta, lane == 0, own);
+            span_grad(p, r.lo, r.hi, r.mid, lane, G, g);
+            if (lane == 0) { t[0] += own[0]; t[1] += own[1]; t[2] += own[2]; }
+        }
+    }
+    if (lane == 0) {
+        double* mine = red + threadIdx.x / G * 3;
+        mine[0] = t[0];
+        mine[1] = t[1];
+        mine[2] = t[2];
+    }
+    __syncthreads();
+    if (threadIdx.x < 3) {
+        double sum = red[threadIdx.x];
+        for (int i = 1; i < PER; ++i) sum += red[i * 3 + threadIdx.x];
+        p.terms[(size_t)blockIdx.x * 3 + threadIdx.x] = sum;
+    }
 }
 
 // Few, long pairs: a block per piece of one; its sum, then (every block joining its pair's pieces, in order) its gradients.
@@ -162,7 +262,7 @@ __global__ __launch_bounds__(256) void k_pref_sums(PrefArgs p) {
     const PairRows r = rows_of_pair(p, blockIdx.x / p.splits);
     long long lo, hi;
     piece_of_pair(p, r, blockIdx.x % p.splits, lo, hi);
-    const double v = wave_sum(span_sum(p, lo, hi, r.mid, threadIdx.x, 256));
+    const double v = group_sum<64>(span_sum(p, lo, hi, r.mid, threadIdx.x, 256));
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     if (threadIdx.x == 0) p.sums[blockIdx.x] = ((red[0] + red[1]) + red[2]) + red[3];
@@ -178,16 +278,16 @@ __global__ __launch_bounds__(256) void k_pref_grad(PrefArgs p) {
     const double* sums = p.sums + (size_t)pair * p.splits;
     double d = 0.0;
     for (int i = lane; i < p.splits; i += 64) d += sums[i];
-    const double g = pair_head(p, pair, wave_sum(d), threadIdx.x == 0 && part == 0, p.terms);
+    const double g = pair_head(p, pair, group_sum<64>(d), threadIdx.x == 0 && part == 0, p.terms + (size_t)pair * 3);
     const PairRows r = rows_of_pair(p, pair);
     long long lo, hi;
     piece_of_pair(p, r, part, lo, hi);
     span_grad(p, lo, hi, r.mid, threadIdx.x, 256, g);
 }
 
-__global__ __launch_bounds__(FINISH_NT) void k_pref_finish(const double* __restrict__ terms, int P, float* __restrict__ loss3) {
+__global__ __launch_bounds__(FINISH_NT) void k_pref_finish(const double* __restrict__ terms, int n, int P, float* __restrict__ loss3) {
     __shared__ double out[3];
-    sum_terms(terms, (size_t)P, out);
+    sum_terms(terms, (size_t)n, out);
     if (threadIdx.x < 3) loss3[threadIdx.x] = (float)(out[threadIdx.x] / (double)P);
 }
 
@@ -596,8 +696,7 @@ __global__ __launch_bounds__(1024) void k_bal_reduce(BalArgs p) {
     const size_t out = (size_t)blockIdx.x * BAL_COLS + c2;
     s = rs[k2][c2];
     n = group_add<32>(rn[k2][c2]);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor(s, o, 64);
+    s = group_sum<32>(s);
     const uint32_t rows = group_add<16>(rv[threadIdx.x & 15]);
     const double inv_v = rows ? 1.0 / (double)rows : 0.0;
     const double mean = s * inv_v, share = (double)n * inv_v / p.K;
@@ -626,6 +725,14 @@ __global__ __launch_bounds__(BAL_NT) void k_bal_grad(BalArgs p) {
     float f[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) f[e] = p.f[off + ln.at(e)];
+    // f less its least entry (in size; all have one sign): f_n - sum f p stays the same, its terms are smaller, and it is zero where
+    // all are equal
+    float least = INFINITY;
+#pragma unroll
+    for (int e = 0; e < E; ++e) least = fminf(least, fabsf(f[e]));
+    least = copysignf(__uint_as_float(group_min<G>(__float_as_uint(least))), (float)p.scale);       // (not negative: ordered as integers)
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] -= least;
     T next[E];
     bool next_on = false;
     if (at.r0 < at.r1) {
@@ -678,7 +785,7 @@ __global__ __launch_bounds__(BAL_NT) void k_bal_grad(BalArgs p) {
         const size_t parts = ((size_t)p.A * p.N + BAL_COLS - 1) / BAL_COLS;
         double t = 0.0;
         for (size_t i = threadIdx.x; i < parts; i += blockDim.x) t += p.terms[i];
-        t = wave_sum(t);
+        t = group_sum<64>(t);
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = t;
         __syncthreads();
         if (threadIdx.x == 0) {
@@ -792,13 +899,20 @@ int pfpn_preference_loss(const float* logp, const float* logp_ref, const float* 
         PFPN_CHECK_LAUNCH();
         return PFPN_OK;
     }
-    if (p.splits == 1) {
+    int left = P;                                       // triples of terms that are left to add up
+    if (p.splits == 1 && T / P <= PREF_SHORT && 3 * (T / P) <= P) {
+        const bool few = T / P <= 128;
+        const int need = few ? (P + 15) / 16 : (P + 3) / 4;
+        left = need < 2048 ? need : 2048;
+        if (few) hipLaunchKernelGGL((k_pref_groups<16>), dim3((unsigned)left + outside), dim3(256), 0, st, p, left);
+        else hipLaunchKernelGGL((k_pref_groups<64>), dim3((unsigned)left + outside), dim3(256), 0, st, p, left);
+    } else if (p.splits == 1) {
         hipLaunchKernelGGL(k_pref_pairs, dim3((unsigned)P + outside), dim3(256), 0, st, p);
     } else {
         hipLaunchKernelGGL(k_pref_sums, dim3(blocks), dim3(256), 0, st, p);
         hipLaunchKernelGGL(k_pref_grad, dim3(blocks + outside), dim3(256), 0, st, p);
     }
-    hipLaunchKernelGGL(k_pref_finish, dim3(1), dim3(FINISH_NT), 0, st, (const double*)p.terms, P, loss3);
+    hipLaunchKernelGGL(k_pref_finish, dim3(1), dim3(FINISH_NT), 0, st, (const double*)p.terms, left, P, loss3);
     PFPN_CHECK_LAUNCH();
     return PFPN_OK;
 }

@@ -303,6 +303,35 @@ def test_preference_loss(dev, T, lengths, kind):
         close(l3, loss3, 2 * U * size + per * float(loss3.abs().max()) + noise * (1 + 20 * float(loss3.abs().max()) ** 0.5), "loss3")
 
 
+@pytest.mark.parametrize("P,longest", [(700, 5), (40000, 4), (2000, 60), (9000, 400), (1100, 350), (200, 1000), (200, 3000), (150, 4095)])
+def test_many_ragged_pairs(dev, P, longest):
+    """every form of the launch by the mean length of a pair; segments of no step among them"""
+    from pfpn_amd import kernels
+    g = torch.Generator()
+    g.manual_seed(P)
+    lengths = torch.randint(0, longest + 1, (2 * P,), generator=g)
+    offsets = torch.cat([torch.tensor([2]), 2 + lengths.cumsum(0)])
+    T = int(offsets[-1]) + 5
+    logp, w = -30 + 3 * torch.randn(T, generator=g), torch.rand(T, generator=g)
+    ref = logp + 0.1 * torch.randn(T, generator=g)
+    w[torch.rand(T, generator=g) < 0.2] = 0.0
+    of = torch.repeat_interleave(torch.arange(2 * P), lengths)
+    gap = ((logp.double() - ref.double()) * w.double())[2:-5]
+    sums = torch.zeros(2 * P, dtype=torch.float64).index_add_(0, of, gap)
+    m = 0.1 * (sums[0::2] - sums[1::2])
+    loss3 = torch.stack([-torch.nn.functional.logsigmoid(m).mean(), (m > 0).double().mean(), m.mean()])
+    want = torch.zeros(T, dtype=torch.float64)
+    want[2:-5] = (-0.1 * torch.sigmoid(-m) / P).repeat_interleave(2)[of] * torch.where(of % 2 == 0, 1.0, -1.0) * w[2:-5].double()
+    d, got, l3 = kernels.preference_loss(*[t.to(dev) for t in (logp, offsets)], logp_ref=ref.to(dev), weight=w.to(dev), beta=0.1)
+    # (bounds as above: sums in 64 bits, the head's 32-bit exponential, logarithm and quotient 16 u, its argument |m| u)
+    noise, per = 2.0 ** -50 * 40 * (2 * longest + 1), 16 * U + U * float(m.abs().max())
+    close(d.cpu(), want, U * want.abs() + 0.1 / P * per + 0.1 * noise + 1e-37, "dlogp")
+    close(got.cpu(), m, U * m.abs() + noise, "margin")
+    close(l3.cpu(), loss3, 2 * U * loss3.abs() + per * float(loss3.abs().max()) + noise + 1e-12, "loss3")
+    again = kernels.preference_loss(*[t.to(dev) for t in (logp, offsets)], logp_ref=ref.to(dev), weight=w.to(dev), beta=0.1)
+    assert torch.equal(d, again[0]) and torch.equal(l3, again[2])
+
+
 def test_preference_gradient_against_differences(dev):
     """central differences of the 64-bit loss, h = 1e-4: off by h^2 beta^3 and 2^-52 / h, under 1e-9"""
     from pfpn_amd import kernels
@@ -432,6 +461,17 @@ def test_balance_gradient_against_differences(dev):
             v.append(float(3.0 * 5 / 2 * (f * torch.softmax(z, -1).mean(0)).sum()))
         num.view(-1)[i] = (v[0] - v[1]) / (2 * h)
     assert float((d.double().cpu() - num).abs().max()) < 2e-6 * float(num.abs().max()) + 1e-9
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,A,N", [(7, 1, 1), (40, 3, 8), (33, 36, 35), (9, 2, 64)])
+def test_equal_counts_leave_no_gradient(dev, R, A, N, dtype):
+    """every category counts in every row: the gradient is zero, not the rounding of two equal terms"""
+    from pfpn_amd import kernels
+    x, _, _ = make_logits(dev, R, A, N, dtype, seed=N)
+    for coef in (0.01, -2.0):
+        loss, counts, _, d = kernels.balance_loss(x, topk=N, coef=coef)
+        assert not d.any() and bool((counts == R).all()) and abs(float(loss) - coef) < 1e-5 * abs(coef)
 
 
 # ---- refusals, empty batches, streams, graphs -------------------------------------------------------------------------------------
