@@ -65,8 +65,8 @@ __device__ __forceinline__ double row_weight(const CatArgs& p, size_t b) {
 // Phase 1: {l_k, m, s} of every segment into LDS; phase 2: the rows' log-probs and loss heads (64 bits), lanes_per_row lanes a
 // row; phase 3: the gradients from the exponentials that phase 1 left in registers (IT segments a group; IT = 0, rows too wide
 // for that: from the logits again, out of the caches).
-// Bound: HBM, one read of the logits and one write of the gradient.  8192 x 128 x 256 float32: 390 us = 5.5 TB/s (a 1-GiB copy on
-// the same card: 425 us); 4096 x 36 x 35: 14.4 us = 2.9 TB/s, one wave of blocks, latency and instructions (13 us of VALU issue).
+// Bound: HBM, one read of the logits and one write of the gradient.  8192 x 128 x 256 float32: 380 us = 5.7 TB/s (a 1-GiB copy on
+// the same card: 425 us); 4096 x 36 x 35: 13.8 us = 3.0 TB/s, one wave of blocks, latency and instructions (13 us of VALU issue).
 // What it measured on the way, 8192 x 128 x 256: reading the logits twice 933 us; holding 64 exponentials a thread, spilled around
 // the 64-bit head, 555 us; loads behind bounds branches (hipcc waits for each one) 511 us; clamped loads without a branch and half
 // of the exponentials parked in LDS 395 us.  Eight lanes x 5 for 35 particles, not 4 x 9: fewer waves, 14.1 against 16.2 us.
