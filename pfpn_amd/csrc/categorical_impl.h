@@ -216,10 +216,17 @@ __global__ __launch_bounds__(NT, E * IT > 32 ? 4 : 8) void k_cat_rows(CatArgs p)
         double lp = 0.0;
         const double w = MODE == CAT_PPO && my_row < rows ? row_weight(p, row0 + my_row) : 1.0;
         if (my_row < rows && w != 0.0) {
+            // one logarithm a lane: of the product of its sums (at most 64 of them, each 0 or within [1, 1024]; 1048 x 4000 x 8: 63 of
+            // them a lane, 129 -> 95 us)
+            double prod = 1.0;
             for (int a = tid % LP; a < p.A; a += LP) {
                 const Segment v = seg[my_row * p.A + a];
-                if (v.k >= 0) lp += v.s == 0.f ? (double)-INFINITY : (double)v.xk - (double)v.m - log((double)v.s);
+                if (v.k >= 0) {
+                    lp += (double)v.xk - (double)v.m;
+                    prod *= (double)v.s;
+                }
             }
+            lp = prod == 0.0 ? (double)-INFINITY : lp - log(prod);
         }
         lp = LP == 1 ? lp : LP == 4 ? group_sum<4>(lp) : LP == 16 ? group_sum<16>(lp) : group_sum<64>(lp);
         if (tid % LP == 0 && my_row < rows) {
@@ -780,7 +787,10 @@ int run_cat(CatArgs p, void* ws, size_t ws_bytes, size_t* nparts, hipStream_t st
     // 2.6 / 3.3 us held, 4.7 / 6.3 us in pieces; of 32768: 3.5 / 5.7 against 4.7 / 6.5; of 65536: 4.8 / 8.9 against 4.8 / 6.7, and
     // 128 rows of 65536: 5.9 / 15.3 against 9.8 / 20.7 us.
     if ((p.A == 1 || MODE == CAT_BWD) && p.N <= 1024 * 16 * V && (S == 1 || p.N <= 32768 || segs >= 128)) {
-        if (p.N <= 256 * 4 * V) launch_held<T, MODE, 4, 256>(p, st);
+        // (fewest idle slots: 32736 x 1025 bfloat16 by 256 threads, most of whose slots are idle: log-prob 63 us, gradient 71 us; by 64 threads 23 and 31 us)
+        if (p.N <= 64 * 4 * V) launch_held<T, MODE, 4, 64>(p, st);
+        else if (p.N <= 128 * 4 * V) launch_held<T, MODE, 4, 128>(p, st);
+        else if (p.N <= 256 * 4 * V) launch_held<T, MODE, 4, 256>(p, st);
         else if (p.N <= 512 * 4 * V) launch_held<T, MODE, 4, 512>(p, st);
         else if (p.N <= 1024 * 4 * V) launch_held<T, MODE, 4, 1024>(p, st);
         else if (p.N <= 1024 * 8 * V) launch_held<T, MODE, 8, 1024>(p, st);
