@@ -58,11 +58,34 @@ __global__ __launch_bounds__(NT) void k_policy_rows(const float* __restrict__ lo
     }
 }
 
+// a wave a term: it reads and writes nothing but its term of the block's FOLD triples
+__global__ __launch_bounds__(192) void k_fold_terms(double* part, size_t n) {
+    const size_t first = (size_t)blockIdx.x * FOLD;
+    const int term = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    double t[FOLD / 64], s = 0.0;
+#pragma unroll
+    for (int k = 0; k < (int)FOLD / 64; ++k) {
+        const size_t j = first + lane + 64 * k;
+        t[k] = part[(j < n ? j : first) * 3 + term];
+    }
+#pragma unroll
+    for (int k = 0; k < (int)FOLD / 64; ++k) s += first + lane + 64 * k < n ? t[k] : 0.0;
+    s = group_sum<64>(s);
+    if (lane == 0) part[first * 3 + term] = s;
+}
+int fold_terms(double* part, size_t& n, hipStream_t st) {
+    if (n <= FOLD_FROM) return 1;
+    const size_t left = (n + FOLD - 1) / FOLD;
+    hipLaunchKernelGGL(k_fold_terms, dim3((unsigned)left), dim3(192), 0, st, part, n);
+    n = left;
+    return (int)FOLD;
+}
+
 // loss4 = {policy + c kl, policy, kl, clipped}: the blocks' sums in a fixed order
-__global__ __launch_bounds__(FINISH_NT) void k_policy_finish(const double* __restrict__ part, size_t nparts, double kl_coef,
+__global__ __launch_bounds__(FINISH_NT) void k_policy_finish(const double* __restrict__ part, size_t nparts, int step, double kl_coef,
                                                              float* __restrict__ loss4) {
     __shared__ double out[3];
-    sum_terms(part, nparts, out);
+    sum_terms(part, nparts, step, out);
     if (threadIdx.x == 0) write_loss4(out, kl_coef, loss4);
 }
 
@@ -87,7 +110,9 @@ static int run_typed(CatArgs p, int dtype, void* ws, size_t ws_bytes, float* los
                  : dtype == DT_BF16 ? run_cat<bf16_t, MODE>(p, ws, ws_bytes, &nparts, st)
                                     : run_cat<f16_t, MODE>(p, ws, ws_bytes, &nparts, st);
     if (rc != PFPN_OK || MODE != CAT_PPO || nparts == 0) return rc;
-    hipLaunchKernelGGL(k_policy_finish, dim3(1), dim3(FINISH_NT), 0, st, (const double*)ws, nparts, p.head.kl_coef, loss4);
+    double* part = static_cast<double*>(ws);
+    const int step = fold_terms(part, nparts, st);
+    hipLaunchKernelGGL(k_policy_finish, dim3(1), dim3(FINISH_NT), 0, st, (const double*)part, nparts, step, p.head.kl_coef, loss4);
     PFPN_CHECK_LAUNCH();
     return PFPN_OK;
 }
@@ -171,7 +196,7 @@ int pfpn_policy_kl_loss(const float* logp, const float* logp_old, const float* a
     } else {
         const int blocks = policy_row_blocks(n);
         hipLaunchKernelGGL((k_policy_rows<256>), dim3(blocks), dim3(256), 0, st, logp, h, (size_t)n, dlogp, part, (float*)nullptr);
-        hipLaunchKernelGGL(k_policy_finish, dim3(1), dim3(FINISH_NT), 0, st, (const double*)part, (size_t)blocks, kl_coef, loss4);
+        hipLaunchKernelGGL(k_policy_finish, dim3(1), dim3(FINISH_NT), 0, st, (const double*)part, (size_t)blocks, 1, kl_coef, loss4);
     }
     PFPN_CHECK_LAUNCH();
     return PFPN_OK;

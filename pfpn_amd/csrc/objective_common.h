@@ -341,9 +341,13 @@ __device__ __forceinline__ void block_terms(const HeadTerms& t, double* red, dou
     }
 }
 
-// n triples of terms added by one block of 15 waves, five a term, sixteen loads of a lane in flight; out[3] in LDS, fixed order
+// n triples of terms, `step` triples apart, added by one block of 15 waves, five a term, sixteen loads of a lane in flight; out[3] in
+// LDS, fixed order.  One CU reads 8190 triples in 5.6 us, 32736 in 19 us, 200000 in 143 us: past FOLD_FROM of them `fold_terms`
+// first adds every FOLD into the first of them (a launch that fills the chip); returns the distance of what is left, n its number.
+constexpr size_t FOLD = 512, FOLD_FROM = 8192;
+int fold_terms(double* part, size_t& n, hipStream_t st);
 constexpr int FINISH_NT = 960;
-__device__ __forceinline__ void sum_terms(const double* __restrict__ part, size_t n, double* out) {
+__device__ __forceinline__ void sum_terms(const double* __restrict__ part, size_t n, int step, double* out) {
     constexpr int LANES = FINISH_NT / 3, DEEP = 16;
     __shared__ double red[15];
     const int wid = threadIdx.x >> 6, lane = threadIdx.x & 63, term = wid % 3;
@@ -353,7 +357,7 @@ __device__ __forceinline__ void sum_terms(const double* __restrict__ part, size_
 #pragma unroll
         for (int k = 0; k < DEEP; ++k) {
             const size_t j = i + LANES * k;
-            t[k] = part[(j < n ? j : i) * 3 + term];
+            t[k] = part[(j < n ? j : i) * step * 3 + term];
         }
 #pragma unroll
         for (int k = 0; k < DEEP; ++k) s += i + LANES * k < n ? t[k] : 0.0;

@@ -285,9 +285,9 @@ __global__ __launch_bounds__(256) void k_pref_grad(PrefArgs p) {
     span_grad(p, lo, hi, r.mid, threadIdx.x, 256, g);
 }
 
-__global__ __launch_bounds__(FINISH_NT) void k_pref_finish(const double* __restrict__ terms, int n, int P, float* __restrict__ loss3) {
+__global__ __launch_bounds__(FINISH_NT) void k_pref_finish(const double* __restrict__ terms, size_t n, int step, int P, float* __restrict__ loss3) {
     __shared__ double out[3];
-    sum_terms(terms, (size_t)n, out);
+    sum_terms(terms, n, step, out);
     if (threadIdx.x < 3) loss3[threadIdx.x] = (float)(out[threadIdx.x] / (double)P);
 }
 
@@ -899,20 +899,22 @@ int pfpn_preference_loss(const float* logp, const float* logp_ref, const float* 
         PFPN_CHECK_LAUNCH();
         return PFPN_OK;
     }
-    int left = P;                                       // triples of terms that are left to add up
+    size_t left = P;                                       // triples of terms that are left to add up
     if (p.splits == 1 && T / P <= PREF_SHORT && 3 * (T / P) <= P) {
         const bool few = T / P <= 128;
         const int need = few ? (P + 15) / 16 : (P + 3) / 4;
-        left = need < 2048 ? need : 2048;
-        if (few) hipLaunchKernelGGL((k_pref_groups<16>), dim3((unsigned)left + outside), dim3(256), 0, st, p, left);
-        else hipLaunchKernelGGL((k_pref_groups<64>), dim3((unsigned)left + outside), dim3(256), 0, st, p, left);
+        const int blocks = need < 2048 ? need : 2048;
+        left = blocks;
+        if (few) hipLaunchKernelGGL((k_pref_groups<16>), dim3((unsigned)blocks + outside), dim3(256), 0, st, p, blocks);
+        else hipLaunchKernelGGL((k_pref_groups<64>), dim3((unsigned)blocks + outside), dim3(256), 0, st, p, blocks);
     } else if (p.splits == 1) {
         hipLaunchKernelGGL(k_pref_pairs, dim3((unsigned)P + outside), dim3(256), 0, st, p);
     } else {
         hipLaunchKernelGGL(k_pref_sums, dim3(blocks), dim3(256), 0, st, p);
         hipLaunchKernelGGL(k_pref_grad, dim3(blocks + outside), dim3(256), 0, st, p);
     }
-    hipLaunchKernelGGL(k_pref_finish, dim3(1), dim3(FINISH_NT), 0, st, (const double*)p.terms, left, P, loss3);
+    const int step = fold_terms(p.terms, left, st);
+    hipLaunchKernelGGL(k_pref_finish, dim3(1), dim3(FINISH_NT), 0, st, (const double*)p.terms, left, step, P, loss3);
     PFPN_CHECK_LAUNCH();
     return PFPN_OK;
 }
