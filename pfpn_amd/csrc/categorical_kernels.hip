@@ -11,8 +11,7 @@ namespace pfpn {
 
 // ---------------------------------------------------------------------------------------------------------------------
 // The same loss on log-probs that come from elsewhere (the particle mixture's own density): one pass over [n] vectors.
-// 1000003 rows, weighted: 7.6 us + 2.3 us for the sum of the blocks (24 MB: 3.7 us at the cache's rate); 11.7 us with the
-// exponentials in 64 bits (80 double instructions a row).
+// 1000003 rows, weighted: 7.6 us + 2.3 us for the sum of the blocks (24 MB: 3.7 us at the cache's rate).
 // ---------------------------------------------------------------------------------------------------------------------
 // Four rows a load, from any alignment.  One block (n <= 4096) finishes the sums itself.
 constexpr long long ROWS_SMALL = 4096;

@@ -253,9 +253,9 @@ struct Axis {
 // ---- the loss head of one row ---------------------------------------------------------------------------------------
 // a = clip((adv - mean) * rstd), r = exp(logp - logp_old), d = logp_ref - logp,
 // loss_row = w (-min(r a, clip(r) a) + c (exp(d) - 1 - d)),   d loss / d logp = w ([not clipped] (-a r) - c (exp(d) - 1)).
-// The differences of the log-probs are taken in 64 bits (a joint log-prob of many dimensions is some hundreds, its difference to
-// the old one some hundredths), their exponentials in 32: off by 2^-24 (|difference| + 3); exp(d) - 1 - d = d^2 / 2 + ... by its
-// series where it would cancel.  The sums over rows are 64-bit.
+// The log-probs of a choice under two policies may lie hundreds apart (a joint log-prob of many dimensions is some hundreds):
+// differences, exponentials and products are 64-bit, so that a ratio beyond float32 under a small weight, or an advantage of zero,
+// gives the loss and gradient it has.  exp(d) - 1 - d = d^2 / 2 + ... by its series where it would cancel.
 struct HeadArgs {
     const float* logp_old;
     const float* adv;
@@ -284,45 +284,47 @@ __device__ __forceinline__ HeadRow head_row(const HeadArgs& h, size_t b) {
     return r;
 }
 
-// exp(d) - 1 - d; em1 = exp(d) - 1.  |d| < 1: d^2 sum_k d^k / (k + 2)!, the first term left out under 2^-28 of the sum
-__device__ __forceinline__ float kl_sample(float d, float& em1) {
-    if (fabsf(d) < 1.f) {
+// exp(d) - 1 - d; em1 = exp(d) - 1.  |d| < 1: d^2 sum_k d^k / (k + 2)!, the sum in 32 bits (a few 2^-24 of itself), the first term left
+// out under 2^-28 of it
+__device__ __forceinline__ double kl_sample(double d, double& em1) {
+    if (fabs(d) < 1.0) {
+        const float x = (float)d;
         float q = 1.f / 6227020800.f;
-        q = __builtin_fmaf(q, d, 1.f / 479001600.f);
-        q = __builtin_fmaf(q, d, 1.f / 39916800.f);
-        q = __builtin_fmaf(q, d, 1.f / 3628800.f);
-        q = __builtin_fmaf(q, d, 1.f / 362880.f);
-        q = __builtin_fmaf(q, d, 1.f / 40320.f);
-        q = __builtin_fmaf(q, d, 1.f / 5040.f);
-        q = __builtin_fmaf(q, d, 1.f / 720.f);
-        q = __builtin_fmaf(q, d, 1.f / 120.f);
-        q = __builtin_fmaf(q, d, 1.f / 24.f);
-        q = __builtin_fmaf(q, d, 1.f / 6.f);
-        q = __builtin_fmaf(q, d, 0.5f);
-        const float kl = q * d * d;
+        q = __builtin_fmaf(q, x, 1.f / 479001600.f);
+        q = __builtin_fmaf(q, x, 1.f / 39916800.f);
+        q = __builtin_fmaf(q, x, 1.f / 3628800.f);
+        q = __builtin_fmaf(q, x, 1.f / 362880.f);
+        q = __builtin_fmaf(q, x, 1.f / 40320.f);
+        q = __builtin_fmaf(q, x, 1.f / 5040.f);
+        q = __builtin_fmaf(q, x, 1.f / 720.f);
+        q = __builtin_fmaf(q, x, 1.f / 120.f);
+        q = __builtin_fmaf(q, x, 1.f / 24.f);
+        q = __builtin_fmaf(q, x, 1.f / 6.f);
+        q = __builtin_fmaf(q, x, 0.5f);
+        const double kl = (double)q * d * d;
         em1 = d + kl;
         return kl;
     }
-    em1 = expf(d) - 1.f;
+    em1 = exp(d) - 1.0;
     return em1 == INFINITY ? em1 : em1 - d;         // (an impossible choice: infinite, not inf - inf)
 }
 
 // -> d loss / d logp of a row of weight != 0; its terms
 __device__ __forceinline__ double policy_head(double logp, const HeadRow& row, const HeadArgs& h, HeadTerms& t) {
-    const float r = expf((float)(logp - (double)row.logp_old));
-    const float lo = (float)h.clip_lo, hi = (float)h.clip_hi;
-    const float held_r = r < lo ? lo : (r > hi ? hi : r);
-    const float sur = r * row.a, held = held_r * row.a;
+    const double r = exp(logp - (double)row.logp_old), a = (double)row.a;
+    const double held_r = r < h.clip_lo ? h.clip_lo : (r > h.clip_hi ? h.clip_hi : r);
+    const double sur = a == 0.0 && r > h.clip_hi ? 0.0 : r * a;        // (no advantage, no surrogate: not inf * 0)
+    const double held = held_r * a;
     const bool clipped = held < sur;
-    double g = clipped ? 0.0 : -(double)sur;
-    float kl = 0.f;
+    double g = clipped ? 0.0 : -sur;
+    double kl = 0.0;
     if (h.logp_ref) {
-        float em1;
-        kl = kl_sample((float)((double)row.logp_ref - logp), em1);
-        if (h.kl_coef != 0.0) g -= h.kl_coef * (double)em1;        // (a term that is only reported may be infinite)
+        double em1;
+        kl = kl_sample((double)row.logp_ref - logp, em1);
+        if (h.kl_coef != 0.0) g -= h.kl_coef * em1;                // (a term that is only reported may be infinite)
     }
-    t.policy = row.w * (clipped ? -(double)held : -(double)sur);
-    t.kl = row.w * (double)kl;
+    t.policy = row.w * (clipped ? -held : -sur);
+    t.kl = row.w * kl;
     t.clipped = clipped ? row.w : 0.0;
     return row.w * g;
 }

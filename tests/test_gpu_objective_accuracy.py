@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from _objectives import U, balance, segment_bound, softmax
+from _objectives import U, balance, gradient, logprob, rounded, segment_bound, softmax
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -46,3 +46,75 @@ def test_balance_gradient_of_nearly_equal_counts(dev, R, A, N, K, dtype):
     ok = between(got[3], grad, bound)
     assert bool(ok.all()), "%d of %d entries, off by up to %.3g of the bound" % (
         int((~ok).sum()), ok.numel(), float(((got[3].double() - grad).abs() / bound).masked_fill(ok, 0).max()))
+
+
+# ---- clipped loss with a KL term: log-probs that lie far apart ------------------------------------------------------------------------
+def far_head(logp, old, adv, ref, w, eps, c, err=0.0):
+    """-> dlogp, its bound, loss4 and its bound, in 64 bits.  The kernels' differences, exponentials and products are 64-bit; the series of
+    the KL term (|d| < 1) has a 32-bit sum: 4 u of itself.  `err`: what the log-prob itself is off by.  A row of advantage 0 has no
+    surrogate, however large its ratio."""
+    a, w = adv.double(), w.double()
+    r = torch.exp(logp - old.double())
+    sur = torch.where(a == 0, torch.zeros_like(r), r * a)
+    held = r.clamp(1 - eps, 1 + eps) * a
+    clipped = held < sur
+    d = ref.double() - logp
+    em1, kl = torch.expm1(d), torch.expm1(d) - d
+    pol, g = torch.where(clipped, -held, -sur), torch.where(clipped, torch.zeros_like(sur), -sur)
+    dlogp = w * (g - c * em1)
+    series = torch.where(d.abs() < 1, kl, torch.zeros_like(kl)).abs()
+    slack = w * ((g.abs() + c * (em1.abs() + 1)) * (1.01 * err) + 4 * U * c * series) + 1e-14 * w * (g.abs() + c * em1.abs())
+    loss4 = torch.stack([(w * t).sum() for t in (pol + c * kl, pol, kl, clipped.double())])
+    part = w * (g.abs() * (1.01 * err) + 4 * U * series) + w * (1.01 * err) * em1.abs() + 1e-14 * w * (pol.abs() + kl)
+    off = torch.stack([part.sum() * (1 + c), part.sum(), part.sum(), 1e-14 * w.sum()])
+    return dlogp, U * dlogp.abs() + slack + 1e-45, loss4, U * loss4.abs() + off + 1e-45
+
+
+GAPS = [-100.0, -88.0, -3.0, -0.25, 0.0, 2.0 ** -7, 0.25, 3.0, 60.0, 88.0, 90.0, 100.0]
+
+
+def test_far_log_probs(dev):
+    """every gap to the old policy with every gap to the reference, under advantages of both signs and none; weights small enough
+    that ratios of e^100 leave finite sums"""
+    from pfpn_amd import kernels
+    gap, ref, adv = [t.reshape(-1) for t in torch.meshgrid(torch.tensor(GAPS), torch.tensor(GAPS), torch.tensor([0.0, 1.5, -0.7]),
+                                                          indexing="ij")]
+    logp = torch.full_like(gap, -256.0)
+    old, ref, w = logp - gap, logp + ref, torch.full_like(gap, 1e-20)
+    # ... and gaps whose ratio no 64-bit number holds, or that are infinite: clipped, or without an advantage
+    extra = torch.tensor([[-256.0, -2000.0, -256.0, 0.0, 1e-20], [-256.0, -2000.0, -256.0, 2.0, 1e-20],
+                          [-256.0, -math.inf, -256.0, 0.0, 1e-20], [-256.0, -math.inf, -256.0, 2.0, 1e-20],
+                          [-256.0, 1000.0, -256.0, -1.0, 1e-20], [-256.0, -256.0, -2000.0, 1.0, 1e-20]]).t()
+    logp, old, ref, adv, w = [torch.cat([t, e]).to(dev) for t, e in zip((logp, old, ref, adv, w), extra)]
+    for n in (logp.shape[0], 5000):            # (one block, which finishes the sums itself, and many)
+        args = [t.repeat(n // logp.shape[0] + 1)[:n].contiguous() for t in (logp, old, adv, ref, w)]
+        want, bound, loss4, off = far_head(args[0].double(), args[1], args[2], args[3], args[4], 0.2, 0.05)
+        assert torch.isfinite(want).all() and torch.isfinite(loss4).all()
+        dlogp, l4 = kernels.policy_kl_loss(args[0], args[1], args[2], logp_ref=args[3], weight=args[4], kl_coef=0.05)
+        assert bool(((dlogp.double() - want).abs() <= bound).all())
+        assert bool(((l4.double() - loss4).abs() <= off).all())
+    # a NaN is not covered up by an advantage of zero
+    bad = torch.tensor([math.nan, -1.0], device=dev)
+    d, l4 = kernels.policy_kl_loss(bad, torch.zeros(2, device=dev), torch.zeros(2, device=dev))
+    assert d[0].isnan() and d[1] == 0 and l4[0].isnan()
+
+
+@pytest.mark.parametrize("shape", [(36, 40, 8), (36, 2, 300), (36, 1, 5000), (600, 1, 1500), (5, 3, 1100), (3, 1, 70001)])
+def test_far_log_probs_from_logits(dev, shape):
+    from pfpn_amd import kernels
+    B, A, N = shape
+    g = torch.Generator(device=dev)
+    g.manual_seed(N)
+    x = torch.randn(B, A, N, device=dev, generator=g)
+    k = torch.randint(0, N, (B, A), device=dev, generator=g)
+    gap = torch.tensor(GAPS, device=dev).repeat(B // len(GAPS) + 1)[:B] if B > 5 else torch.tensor([100.0, 90.0, 95.0, -90.0, 0.0], device=dev)[:B]
+    adv = torch.tensor([0.0, 1.5, -0.7], device=dev).repeat(B)[:B].roll(1) * (torch.arange(B, device=dev) % 7 != 0)
+    base = kernels.categorical_logprob_fwd(x, k)
+    old, ref, w = base - gap, base + gap.flip(0), torch.full((B,), 1e-20, device=dev)
+    logp, err = logprob(x, k)
+    got = kernels.categorical_ppo_fwd_bwd(x, k, old, adv, logp_ref=ref, weight=w, kl_coef=0.05)
+    dlogp, derr, loss4, off = far_head(logp, old, adv, ref, w, 0.2, 0.05, err)
+    assert torch.isfinite(dlogp).all()
+    want, bound = gradient(x, k, dlogp, derr)
+    assert bool(((got["dlogits"].double() - want).abs() <= rounded(want, bound, torch.float32)).all())
+    assert bool(((got["loss4"].double() - loss4).abs() <= off).all())
