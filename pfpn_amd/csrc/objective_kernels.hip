@@ -97,16 +97,16 @@ __device__ __forceinline__ void outside_zero(const PrefArgs& p, long long id, lo
 // loss of one pair -> d loss / d delta (of the mean); fills its terms[3] and margin when `write`
 __device__ __forceinline__ double pair_head(const PrefArgs& p, int pair, double delta, bool write, double* terms) {
     const double m = p.beta * delta;
-    double loss, slope;
+    double loss = 0.0, slope;
     if (p.kind == 0) {
-        // log sigma(m) = -softplus(-m); both halves from ONE exponential of -|m|, in 32 bits (off by a few 2^-24 of themselves)
-        const float e = (float)p.smoothing, am = fabsf((float)m);
-        const float z = expf(-am), l = log1pf(z), near = 1.f / (1.f + z), far = z * near;
-        const float good = m >= 0 ? near : far, bad = m >= 0 ? far : near;
-        const float sp_neg = l + (m < 0 ? am : 0.f), sp_pos = l + (m > 0 ? am : 0.f);
-        loss = (1.f - e) * sp_neg + (e > 0.f ? e * sp_pos : 0.f);      // (an infinite margin: 0, not 0 * inf)
-        slope = p.beta * (double)(e * good - (1.f - e) * bad);
-        if (m != m) { loss = m; slope = m; }
+        // log sigma(m) = -softplus(-m); both halves from ONE exponential of -|m|.  In 64 bits: e sigma(m) - (1 - e) sigma(-m) cancels
+        // near its zero, and an exponential in 32 is off by |m| 2^-24 of itself
+        const double e = p.smoothing, am = fabs(m), z = exp(-am), near = 1.0 / (1.0 + z), far = z * near;
+        slope = p.beta * (m >= 0 ? e * near - (1.0 - e) * far : e * far - (1.0 - e) * near);
+        if (write) {
+            const double l = log1p(z);
+            loss = (1.0 - e) * (l + (m < 0 ? am : 0.0)) + (e > 0 ? e * (l + (m > 0 ? am : 0.0)) : 0.0);   // (infinite margin: 0, not 0 * inf)
+        }
     } else {
         const double u = delta - 0.5 / p.beta;
         loss = u * u;

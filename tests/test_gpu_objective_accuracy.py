@@ -118,3 +118,48 @@ def test_far_log_probs_from_logits(dev, shape):
     want, bound = gradient(x, k, dlogp, derr)
     assert bool(((got["dlogits"].double() - want).abs() <= rounded(want, bound, torch.float32)).all())
     assert bool(((got["loss4"].double() - loss4).abs() <= off).all())
+
+
+# ---- preference loss: pairs that are won or lost by far, and slopes that cancel ----------------------------------------------------------
+# P pairs of 2 L steps: the one-block form, groups of 16 and 64 lanes, a block a pair (held and not), pieces of a pair
+@pytest.mark.parametrize("P,L", [(12, 3), (2000, 8), (1500, 200), (300, 300), (400, 1000), (2, 20000)])
+@pytest.mark.parametrize("kind,smoothing", [("logistic", 0.0), ("logistic", 0.02), ("logistic", 0.5), ("squared", 0.0)])
+def test_preference_of_far_margins(dev, P, L, kind, smoothing):
+    """the slope -(1 - e) sigma(-m) + e sigma(m) where it is e^-|m| and where it is a small difference: beside its rounding nothing of 32
+    bits is in it"""
+    from pfpn_amd import kernels
+    margins = torch.tensor([-80.0, -20.0, -3.0, -1e-3, 0.0, 1e-6, 0.4, 3.8918202981106265, 12.0, 30.0, 60.0, 85.0])
+    g = torch.Generator()
+    g.manual_seed(P)
+    beta, T = 0.5, 2 * P * L
+    ref = (-8 + torch.randn(T, generator=g)).float()
+    first = margins.repeat(P // len(margins) + 1)[:P] / beta
+    gap = torch.zeros(P, 2, L)
+    gap[:, 0, L // 2] = first
+    gap = gap + torch.randn(P, 2, L, generator=g) * 1e-6
+    logp = (ref.double() + gap.view(-1).double()).float()
+    offsets = torch.arange(2 * P + 1) * L
+    d = (logp.double() - ref.double()).view(P, 2, L).sum(-1)
+    delta = d[:, 0] - d[:, 1]
+    m = beta * delta
+    if kind == "logistic":
+        # (e sigma(m) - (1 - e) sigma(-m) = sigma(-m) (e (1 + e^m) - 1), without a difference of the two)
+        s = torch.where(m < 30, torch.sigmoid(-m) * (smoothing * torch.expm1(m) + (2 * smoothing - 1)),
+                        smoothing * torch.sigmoid(m) - (1 - smoothing) * torch.exp(-m) / (1 + torch.exp(-m)))
+        slope, part = beta * s, beta * (smoothing * torch.sigmoid(m) + (1 - smoothing) * torch.sigmoid(-m))
+        loss = -(1 - smoothing) * torch.nn.functional.logsigmoid(m) - smoothing * torch.nn.functional.logsigmoid(-m)
+    else:
+        slope, loss = 2 * (delta - 0.5 / beta), (delta - 0.5 / beta) ** 2
+        part = slope.abs() + 1 / beta
+    # 64-bit sums of 2 L terms of about 10, their effect on the slope (Lipschitz beta part, or 2), and 64-bit rounding of its parts
+    noise = 2.0 ** -51 * (40 + 2 * L)
+    off = ((beta * part * noise if kind == "logistic" else 2 * noise) + 2.0 ** -48 * part) / P
+    want = slope / P
+    got, margin, l3 = kernels.preference_loss(logp.to(dev), offsets.to(dev), logp_ref=ref.to(dev), beta=beta, label_smoothing=smoothing,
+                                              kind=kind)
+    got = got.double().cpu().view(P, 2, L)
+    bound = (U * want.abs() + off + 1e-45).view(P, 1, 1)
+    assert bool(((got[:, :1] - want.view(P, 1, 1)).abs() <= bound).all()) and bool(((got[:, 1:] + want.view(P, 1, 1)).abs() <= bound).all())
+    assert bool(((margin.double().cpu() - m).abs() <= U * m.abs() + beta * noise).all())
+    mean = loss.mean()
+    assert abs(float(l3[0]) - float(mean)) <= float((U + 2.0 ** -40) * mean + noise * part.mean() * (1 if kind == "logistic" else 200))
