@@ -174,6 +174,7 @@ class ParticleFilteringA2CNetwork(A2CNetwork):
         self.adv_stats = kernels.new_adv_stats(dev, self.clip_advantage)     # {mean, rstd | clip bounds}
         self.ws_mix = kernels.mixture_workspace(B, self.n_actions, self.particles, dev)   # private: deferred finalize
         self._mix_slabs = {}
+        self._defer_ok = {}           # (with the slabs it speaks of: a size that comes back after its buffers were dropped fills both)
         self._pbias_ws = {}
         if self.trunk is not None:
             self.dh = torch.empty(2, B, hc, dtype=torch.float32, device=dev)

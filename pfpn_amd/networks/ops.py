@@ -144,6 +144,7 @@ class DenseStack:
         self.pinned = set()       # batch sizes a captured graph points at (the network shares its set): never dropped
 
     MAX_BUFFER_SETS = 64
+    FORWARD_ONLY = "reference"      # the slot of passes that no backward follows (a frozen policy's): no gradient buffers
 
     def group_view(self, t, layer, g, bias=False):
         """group g's slice of a layer tensor (parameter, gradient or Adam slot) in the reference's shape."""
@@ -183,7 +184,7 @@ class DenseStack:
             t = torch.empty(G, B, H, dtype=torch.float32, device=dev)
             return t.view(G * B, H), t
         a = [alloc(i) for i in range(self.L)]
-        d = [alloc(i) for i in range(self.L)]
+        d = [alloc(i) for i in range(self.L)] if slot != self.FORWARD_ONLY else []
         if len(self._bufs) > self.MAX_BUFFER_SETS:
             # ragged batches (episodic V-trace / A2C rounds) would otherwise keep one activation set per size ever seen:
             # drop the oldest set no graph can point at (a step over B rows may run its stacks over 2B rows: SAC)

@@ -263,3 +263,34 @@ def test_index_log_prob_of_drawn_particles(dev):
     base = torch.ones(20, A * N, device=dev)
     d.balance(coef=2.0, dlogits=base)
     assert float((base - 1 - grad).abs().max()) < 2e-7
+
+
+@pytest.mark.parametrize("particles", [8, 72])
+def test_ppo_steps_after_preference_steps_of_many_lengths(dev, monkeypatch, particles):
+    """more sizes than the network keeps buffers for pass between two eager PPO steps of one size: the second step is the first's
+    form, and leaves the bits of the launch-per-piece steps"""
+    from pfpn_amd.models import SyncReplicasApplier
+    monkeypatch.setenv("PFPN_GRAPH_TRAIN", "0")
+    nets, opts = [], []
+    for defer in (True, False):
+        nets.append(make(dev, particles=particles))
+        spread_out(nets[-1], 6)
+        nets[-1].set_reference()
+        nets[-1].defer_reduce = defer
+        opts.append(SyncReplicasApplier(nets[-1], [{"names": None, "lr": 1e-3}], norm_clip=1.0, world_size=1, fused_norm=False))
+
+    def ppo(seed):
+        b = batch(32, seed)
+        lp = np.random.default_rng(seed).normal(-4, .3, 32).astype(np.float32)
+        return [n.train(None, o, [], b["state"], b["action"], b["value"], lp, b["advantage"]) for n, o in zip(nets, opts)]
+    first = ppo(1)
+    assert nets[0]._defer_ok[(32, True)] is True and first[0] == first[1]
+    for i in range(10):
+        T = 40 + 4 * i
+        b = batch(T, 20 + i)
+        got = [n.train_preference(None, o, [], b["state"], b["action"], [0, 10, 25, 31, T]) for n, o in zip(nets, opts)]
+        assert got[0] == got[1]
+    assert 32 not in nets[0]._buf_cache                     # (its buffers were dropped on the way)
+    again = ppo(2)
+    assert nets[0]._defer_ok[(32, True)] is True and again[0] == again[1]
+    assert torch.equal(nets[0].store.flat, nets[1].store.flat)
