@@ -107,7 +107,7 @@ class ParticleFilteringA2CNetwork(A2CNetwork):
             raise ValueError("balance_beta: at most 1024 particles")
         if not 0.0 < self.preference_beta < float("inf") or not 0.0 <= self.preference_smoothing <= 0.5:
             raise ValueError("preference_beta > 0 and preference_smoothing in [0, 0.5] are needed")
-        self._reference = None
+        self._reference = self._reference_norm = None
 
     # -- parameters ------------------------------------------------------------------------------
     def build_policy_params(self, store, in_dim):
@@ -251,18 +251,29 @@ class ParticleFilteringA2CNetwork(A2CNetwork):
 
     # -- a frozen copy of the policy -------------------------------------------------------------------
     def set_reference(self):
-        """Freeze the policy as it is now (trunk, head, particles) as the reference of the KL term (`kl_coef`) and of
-        train_preference.  Not part of a checkpoint: call it again after restoring one.  Steps captured earlier follow."""
+        """Freeze the policy as it is now (trunk, head, particles, and the state normaliser's mean and deviation, which the live policy
+        goes on moving) as the reference of the KL term (`kl_coef`) and of train_preference.  Steps captured earlier follow.  Not part
+        of a checkpoint: after restoring one call it again (to take up an earlier reference: restore the checkpoint of that time,
+        call it, then restore the latest)."""
+        nz = self.state_normalizer
         if self._reference is None:
             self._reference = self.store.flat.clone()
+            self._reference_norm = (nz.mean.clone(), nz.std.clone()) if nz is not None else None
         else:
             self._reference.copy_(self.store.flat)
+            if nz is not None:
+                for frozen, live in zip(self._reference_norm, (nz.mean, nz.std)):
+                    frozen.copy_(live)
 
-    def _reference_log_prob(self, x, action):
-        """log-prob [B] of `action` under the frozen policy on the normalised states x."""
-        ref = self.store.views_of(self._reference)
+    def _reference_log_prob(self, state, action):
+        """log-prob [B] of `action` under the frozen policy on the raw states."""
+        ref, x = self.store.views_of(self._reference), state
+        if self.normalize_state:
+            x = kernels.state_norm(state, *self._reference_norm, self.clip_state or 0.0)
+        elif self.clip_state:
+            x = torch.clamp(state, -self.clip_state, self.clip_state)
         stack = self.trunk if self.trunk is not None else self.actor_trunk
-        ha = stack.forward(x, slot="reference", params=ref)[0]
+        ha = stack.forward(x, slot=stack.FORWARD_ONLY, params=ref)[0]
         logits = torch.addmm(ref["actor/fc_policy/bias"], ha, ref["actor/fc_policy/weight"])
         return MixtureGaussianDistribution(logits, ref["actor/samples"], ref["actor/samples_std"],
                                            self.normalize_policy_output_).log_prob(action)
@@ -280,7 +291,7 @@ class ParticleFilteringA2CNetwork(A2CNetwork):
         self._ensure_buffers(B)
         deferred = self._deferred_jobs(B)
         x = self.prologue(state, deferred=deferred)
-        logp_ref = self._reference_log_prob(x, action) if self._reference is not None else None
+        logp_ref = self._reference_log_prob(state, action) if self._reference is not None else None
         st = self.store
         if deferred is not None:
             ha, hc = self._trunks_forward(x, value_head=(st["critic/fc3/weight"], st["critic/fc3/bias"], self.value_buf),

@@ -56,7 +56,7 @@ def clip_ppo_network_wrapper(a2c_base_class):
             self._ensure_buffers(B)
             deferred = self._deferred_jobs(B, fused_mixture=True)
             x = self.prologue(state, advantage, deferred=deferred)   # normalised state, state-norm EMA, advantage moments
-            logp_ref = self._reference_log_prob(x, action) if self.kl_coef else None
+            logp_ref = self._reference_log_prob(state, action) if self.kl_coef else None
             w3, b3 = st["critic/fc3/weight"], st["critic/fc3/bias"]
             if deferred is not None:
                 ha, hc = self._trunks_forward(x, value_head=(w3, b3, self.value_buf), masks=True)

@@ -294,3 +294,57 @@ def test_ppo_steps_after_preference_steps_of_many_lengths(dev, monkeypatch, part
     again = ppo(2)
     assert nets[0]._defer_ok[(32, True)] is True and again[0] == again[1]
     assert torch.equal(nets[0].store.flat, nets[1].store.flat)
+
+
+def normalised(s, mean, std, clip=5.0):
+    return torch.clamp((s - mean.double().cpu()) / std.double().cpu(), -clip, clip)
+
+
+@pytest.mark.parametrize("graphs", ["0", "1"])
+def test_reference_keeps_its_normaliser(dev, monkeypatch, graphs):
+    """learner steps on shifted states move the live normaliser: the frozen policy goes on seeing raw states as it did when it was
+    frozen, in the KL term and in preference steps, until set_reference() is called again"""
+    from pfpn_amd.models import SyncReplicasApplier
+    monkeypatch.setenv("PFPN_GRAPH_TRAIN", graphs)
+    net = make(dev, kl_coef=0.3, preference_beta=0.7)
+    spread_out(net, 7)
+    nz = net.state_normalizer
+    g = torch.Generator().manual_seed(3)
+    nz.mean.copy_(0.6 * torch.rand(S, generator=g) - 0.3)
+    nz.std.copy_(0.8 + 0.5 * torch.rand(S, generator=g))
+    opt = SyncReplicasApplier(net, [{"names": None, "lr": 1e-3}], norm_clip=1.0, world_size=1)
+    net.set_reference()
+    for freeze in (False, True):
+        if freeze:
+            net.set_reference()
+        frozen, mean, std = doubles(net, False), nz.mean.clone(), nz.std.clone()
+        for i in range(8):
+            b = batch(32, 30 + i)
+            lp = np.random.default_rng(i).normal(-4, .3, 32).astype(np.float32)
+            net.train(None, opt, [], b["state"] * 2 + 1, b["action"], b["value"], lp, b["advantage"])
+        assert float((nz.mean - mean).abs().max()) > 0.3 and (graphs == "0" or net._train_graphs)
+        # a preference step's loss and gradient, and a PPO step's, from the raw states
+        B, b = 32, batch(32, 50)
+        s, act = torch.from_numpy(b["state"]).double(), torch.from_numpy(b["action"]).double()
+        at = [torch.from_numpy(t).to(dev) for t in (b["state"], b["action"])]
+        with torch.no_grad():
+            ref = twin(frozen, normalised(s, mean, std), act)[2]
+        params, x = doubles(net), normalised(s, nz.mean, nz.std)
+        gap = twin(params, x, act)[2] - ref
+        m = 0.7 * (gap[:9].sum() - gap[9:20].sum())
+        (-torch.nn.functional.logsigmoid(m)).backward()
+        loss3 = net.compute_preference_gradients(*at, torch.tensor([0, 9, 20], device=dev))
+        assert abs(float(loss3[2]) - float(m.detach())) < 1e-4 * (1 + abs(float(m.detach())))
+        compare(net, params, "preference")
+        opt.apply(net)
+        params, x = doubles(net), normalised(s, nz.mean, nz.std)
+        _, v, logp = twin(params, x, act)
+        old = logp.detach().float()
+        adv = torch.from_numpy(b["advantage"]).double()
+        na = (adv - adv.mean()) / (adv.std(unbiased=False) + 1e-8)
+        r, d = torch.exp(logp - old.double()), ref - logp
+        loss = -(r * na).mean() + 0.3 * (torch.expm1(d) - d).mean() + 0.5 * ((v - (adv + torch.from_numpy(b["value"]).double())) ** 2).mean()
+        loss.backward()
+        net.compute_gradients(*at, torch.from_numpy(b["value"]).to(dev), old.to(dev), torch.from_numpy(b["advantage"]).to(dev))
+        compare(net, params, "ppo")
+        opt.apply(net)
