@@ -147,8 +147,8 @@ class ParticleFilteringA2CNetwork(A2CNetwork):
             self.train_ops.append(self.resample_tick)
         else:
             self.max_active = self.sum_active = None
-        if self.trainable and self.balance_beta:
-            # (loss, counts, mean weights) of the latest learner step, also where it was a replay
+        if self.trainable and self.particles <= 1024:
+            # balance loss: (loss, counts, mean weights) of the latest learner step, also where it was a replay
             self.balance_out = (torch.zeros(1, dtype=torch.float32, device=self.device),
                                 torch.zeros(A, N, dtype=torch.int32, device=self.device),
                                 torch.zeros(A, N, dtype=torch.float32, device=self.device))

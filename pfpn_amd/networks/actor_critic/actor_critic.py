@@ -355,6 +355,8 @@ class ActorCriticNetwork(object):
                 return g()
             args = [a.index_select(0, rows) for a in args]
         if g is None:
+            if len(self._train_calls) >= 256:        # (a coefficient annealed at every step: a new key each)
+                self._train_calls.clear()
             n = self._train_calls[key] = self._train_calls.get(key, 0) + 1
             if n > 4 and self.device.type == "cuda" and len(self._train_graphs) < 4 and \
                     os.environ.get("PFPN_GRAPH_TRAIN", "1") != "0":

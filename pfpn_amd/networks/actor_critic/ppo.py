@@ -51,6 +51,8 @@ def clip_ppo_network_wrapper(a2c_base_class):
             No host synchronisation: capturable in a hipGraph."""
             if self.kl_coef and self._reference is None:
                 raise RuntimeError("kl_coef needs a reference policy: call set_reference() first")
+            if self.kl_coef and self.normalize_policy_output_:
+                raise NotImplementedError("kl_coef with a tanh policy is not built (no PPO setting has one)")
             B = state.shape[0]
             st = self.store
             self._ensure_buffers(B)
@@ -105,6 +107,12 @@ def clip_ppo_network_wrapper(a2c_base_class):
                 self._add_balance(out["loss3"])        # (after the launch that finishes the loss)
             return out["loss3"]
 
+        def _graph_phase(self):
+            """a captured step holds the coefficients of its extra terms: one of other coefficients (annealed, switched on or off)
+            is another step (captured after as many eager ones, while there is room for its graph: `graphed_train`)"""
+            extra = (self.kl_coef, self.balance_beta or 0.0)
+            return extra if any(extra) else ()
+
         def _kl_composition(self, policy, action, logp_ref, log_prob, advantage, v, value, dbias):
             """The step's loss with its KL term as launches of its own: log-probs -> clipped loss + KL (kernels.policy_kl_loss)
             and value loss -> the mixture's backward.  Same outputs as the fused kernel; loss3 = {loss, policy loss with its KL
@@ -157,17 +165,18 @@ def clip_ppo_network_wrapper(a2c_base_class):
             size exists (the first steps of a run stay eager, as in graphed_train); the staged rollout lives in static
             device columns the graph's gathers read, so a round of another size gets its own graph (at most two are
             kept).  PFPN_GRAPH_TRAIN=0 (no captured steps at all) keeps rounds eager too."""
-            if (B, id(optimizer)) not in self._train_graphs:
+            step = (B, id(optimizer)) + tuple(self._graph_phase())
+            if step not in self._train_graphs:
                 return None
             in_graph = False
             if getattr(optimizer, "exchange", optimizer.world > 1):
                 # a K-step replay needs the collective INSIDE the graph (the default over RCCL); where the one-step graph of
                 # this size fell back to two graphs around an eager all-reduce, DP rounds run one-step replays
-                in_graph = getattr(self._train_graphs[(B, id(optimizer))], "in_graph_exchange", False)
+                in_graph = getattr(self._train_graphs[step], "in_graph_exchange", False)
                 if not in_graph:
                     return None
             n = cols[0].shape[0]
-            key = (B, n, K, id(optimizer))
+            key = (B, n, K, id(optimizer)) + tuple(self._graph_phase())
             rg = self._round_graphs.get(key) if hasattr(self, "_round_graphs") else None
             if rg is None:
                 if not hasattr(self, "_round_graphs"):
@@ -197,7 +206,8 @@ def clip_ppo_network_wrapper(a2c_base_class):
                         for rows in plan]
             B0, K = len(plan[0]), self.ROUND_STEPS_PER_REPLAY
             n_rows = len(columns[names[0]])
-            rg = getattr(self, "_round_graphs", {}).get((B0, n_rows, K, id(optimizer))) if len(plan) >= K else None
+            rg = getattr(self, "_round_graphs", {}).get((B0, n_rows, K, id(optimizer)) + tuple(self._graph_phase())) \
+                if len(plan) >= K else None
             if rg is not None and all(isinstance(columns[k], np.ndarray) for k in names):
                 # the round's graph exists: the host columns go straight into the static columns its gathers read
                 cols = rg.gather_from[0]

@@ -348,3 +348,37 @@ def test_reference_keeps_its_normaliser(dev, monkeypatch, graphs):
         net.compute_gradients(*at, torch.from_numpy(b["value"]).to(dev), old.to(dev), torch.from_numpy(b["advantage"]).to(dev))
         compare(net, params, "ppo")
         opt.apply(net)
+
+
+@pytest.mark.parametrize("round_rows", [0, 512])
+def test_coefficients_changed_after_the_capture(dev, monkeypatch, round_rows):
+    """kl_coef and balance_beta annealed, switched off and on again between learner steps: replayed steps follow, with eager steps' bits"""
+    from pfpn_amd.models import SyncReplicasApplier
+    got = []
+    for graphs in ("0", "1"):
+        monkeypatch.setenv("PFPN_GRAPH_TRAIN", graphs)
+        net = make(dev, kl_coef=0.2, balance_beta=0.1 if round_rows else None)
+        spread_out(net, 4)
+        net.set_reference()
+        opt = SyncReplicasApplier(net, [{"names": None, "lr": 1e-3}], norm_clip=1.0, world_size=1)
+        losses = []
+        for kl, balance in ((0.2, None), (0.9, None), (0.9, 0.5), (0.0, None), (0.2, None)):
+            net.kl_coef, net.balance_beta = kl, balance
+            if round_rows:
+                b = batch(round_rows, 2)
+                b["log_prob"] = np.random.default_rng(0).normal(-4, .3, round_rows).astype(np.float32)
+                for r in range(2):
+                    plan = [np.random.default_rng(r * 10 + i).permutation(round_rows)[:32] for i in range(16)]
+                    losses += [l for l, _ in net.train_round(opt, [], ["state", "action", "value", "log_prob", "advantage"], b, plan)]
+            else:
+                for it in range(8):
+                    b = batch(32, it)
+                    lp = np.random.default_rng(it).normal(-4, .3, 32).astype(np.float32)
+                    losses.append(net.train(None, opt, [], b["state"], b["action"], b["value"], lp, b["advantage"])[0])
+            if balance:
+                assert int(net.balance_out[1].sum()) == 32 * A
+        got.append((losses, {k: v.clone() for k, v in net.variables().items()}))
+    assert len(net._train_graphs) == 4
+    assert got[0][0] == got[1][0]
+    for k, v in got[0][1].items():
+        assert torch.equal(v, got[1][1][k]), k
