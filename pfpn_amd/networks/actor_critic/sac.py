@@ -43,6 +43,11 @@ def sac_network_wrapper(base_class):
             self.tau = tau
             self.reward, self.not_terminal = "reward", "not_terminal"
 
+        def compute_preference_gradients(self, *args, **kwargs):
+            raise NotImplementedError("train_preference belongs to the policy-gradient networks (PPO, A2C, V-trace)")
+
+        train_preference = compute_preference_gradients
+
         # -- parameters: critic tensors first, then actor tensors (the two Adam groups) ------------
         def _declare(self, store):
             A = int(self.action_shape[0])

@@ -109,3 +109,14 @@ def test_network_options():
     for cls in ("ParticleFilteringSACNetwork", "ParticleFilteringDDPGNetwork"):
         with pytest.raises(NotImplementedError, match="balance_beta"):
             getattr(networks, cls)(**base, balance_beta=0.1)
+
+
+@pytest.mark.parametrize("cls", ["ParticleFilteringSACNetwork", "ParticleFilteringDDPGNetwork"])
+def test_networks_without_a_value_trunk_refuse_preference_steps(cls):
+    """before anything of the step has happened (these networks' critics are Q functions: the step has no place for them)"""
+    from pfpn_amd import networks
+    net = getattr(networks, cls)(trainable=True, state_shape=[5], action_shape=[2], action_lower_bound=[-1, -1],
+                                 action_upper_bound=[1, 1], common_net_shape=[], critic_net_shape=[8], actor_net_shape=[8])
+    for call in (net.compute_preference_gradients, lambda *a: net.train_preference(None, None, [], *a)):
+        with pytest.raises(NotImplementedError, match="train_preference"):
+            call(torch.zeros(4, 5), torch.zeros(4, 2), torch.tensor([0, 2, 4]))
