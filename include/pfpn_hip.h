@@ -254,7 +254,8 @@ int pfpn_policy_kl_loss(const float* logp, const float* logp_old, const float* a
                         const float* weight, const float* adv_stats, long long n, double clip_eps_low, double clip_eps_high,
                         double kl_coef, float* dlogp, float* loss4, void* workspace, size_t workspace_bytes, void* stream);
 /* Loss over P pairs of compared segments (paired log ratios; offsets as pfpn_gae's: segment s = rows [offsets[s],
- * offsets[s+1]) of the T log-probs, DEVICE int64 [2P+1], ascending, clamped to [0, T]; pair p prefers segment 2p to 2p+1):
+ * offsets[s+1]) of the T log-probs, DEVICE int64 [2P+1], ascending; clamped to [0, T] and to
+ * ascend within a pair; pair p prefers segment 2p to 2p+1):
  *   S_s = sum_t w_t (logp_t - logp_ref_t), delta = S_2p - S_2p+1, margin = beta delta,
  *   kind 0: -(1 - e) log sigma(margin) - e log sigma(-margin) (e = label_smoothing); kind 1: (delta - 1 / (2 beta))^2; mean over P.
  * logp_ref, weight optional; a step of weight 0 is skipped whatever it holds.  dlogp [T] is written for every row (0 outside all

@@ -32,7 +32,8 @@ struct PrefArgs {
 };
 
 // A pair's two segments lie side by side: rows [lo, mid) count for it, [mid, hi) against it.  Bounds are clamped to the vectors
-// (and to ascend), so that nothing outside is touched whatever they hold.
+// and to ascend within the pair, so that nothing outside is touched whatever they hold (bounds that descend from one pair to the
+// next make pairs share rows, whose gradient is then one of theirs).
 struct PairRows {
     long long lo, mid, hi;
 };
@@ -87,11 +88,11 @@ __device__ __forceinline__ void span_grad(const PrefArgs& p, long long lo, long 
     const long long t = full + id;
     if (t < hi) p.dlogp[t] = step_grad(t >= mid ? -g : g, p.weight ? p.weight[t] : 1.f);
 }
-// rows outside every segment have no gradient
+// rows outside every segment, before the first pair's and behind the last pair's, have no gradient
 __device__ __forceinline__ void outside_zero(const PrefArgs& p, long long id, long long n) {
-    const long long first = p.offsets[0] < 0 ? 0 : p.offsets[0], last = p.offsets[2 * (size_t)p.P];
-    for (long long t = id; t < first && t < p.T; t += n) p.dlogp[t] = 0.f;
-    for (long long t = (last < 0 ? 0 : last) + id; t < p.T; t += n) p.dlogp[t] = 0.f;
+    const long long first = rows_of_pair(p, 0).lo, last = rows_of_pair(p, p.P - 1).hi;
+    for (long long t = id; t < first; t += n) p.dlogp[t] = 0.f;
+    for (long long t = last + id; t < p.T; t += n) p.dlogp[t] = 0.f;
 }
 
 // loss of one pair -> d loss / d delta (of the mean); fills its terms[3] and margin when `write`

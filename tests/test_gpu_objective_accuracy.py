@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from _objectives import U, balance, gradient, logprob, rounded, segment_bound, softmax
+from _objectives import U, balance, gradient, logprob, preference, rounded, segment_bound, softmax
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -163,3 +163,29 @@ def test_preference_of_far_margins(dev, P, L, kind, smoothing):
     assert bool(((margin.double().cpu() - m).abs() <= U * m.abs() + beta * noise).all())
     mean = loss.mean()
     assert abs(float(l3[0]) - float(mean)) <= float((U + 2.0 ** -40) * mean + noise * part.mean() * (1 if kind == "logistic" else 200))
+
+
+@pytest.mark.parametrize("T", [50, 20001])          # (one block; pieces of a pair)
+def test_preference_bounds_out_of_order(dev, T):
+    """bounds beyond the vector or below the one before: as if clamped to [0, T] and to ascend, the same in every call, and nothing
+    beside the vectors is read (NaN there) or written"""
+    from pfpn_amd import kernels
+    g = torch.Generator(device=dev)
+    g.manual_seed(T)
+    held = [torch.full((T + 64,), math.nan, device=dev) for _ in range(3)]
+    logp, ref, w = [t[32:32 + T] for t in held]
+    logp.normal_(generator=g)
+    ref.normal_(generator=g)
+    w.uniform_(generator=g)
+    s = T // 50
+    for bounds, clamped in (([0, 40, 10], [0, 40, 40]), ([-7, 20, 1 << 40], [0, 20, 50]), ([60, 70, 80], [50, 50, 50]), ([30, 10, 40], [30, 30, 40]),
+                            ([-9, -5, -1], [0, 0, 0]), ([45, 20, 3], [45, 45, 45]), ([1 << 62, -(1 << 62), 0], [50, 50, 50]),
+                            ([0, 10, 30, 45, 20], [0, 10, 30, 45, 45])):
+        scale = lambda v: T if v == 50 else v * s if abs(v) < 1000 else v
+        at = torch.tensor([scale(v) for v in bounds], device=dev)
+        want, margin, _ = preference(logp, torch.tensor([scale(v) for v in clamped], device=dev), ref, w, 0.1, 0.0, "logistic")
+        for _ in range(5):
+            d, m, l3 = kernels.preference_loss(logp, at, logp_ref=ref, weight=w)
+            assert bool(((d.double() - want).abs() <= U * want.abs() + 1e-9 / (len(bounds) // 2) + 1e-37).all()), bounds
+            assert bool(((m.double() - margin).abs() <= U * margin.abs() + 1e-9).all()) and bool(torch.isfinite(l3).all())
+        assert all(bool(t[:32].isnan().all()) and bool(t[-32:].isnan().all()) for t in held)
