@@ -609,6 +609,16 @@ def _logit_grad(dlogits, logits):
     return dlogits, ptr, ld
 
 
+def _apart(out, name, *others):
+    """an output that was given must not lie on memory that other blocks of the launch still read"""
+    lo, hi = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
+    for t in others:
+        if t is not None and t.numel() and t.data_ptr() < hi:
+            last = sum((n - 1) * k for n, k in zip(t.shape, t.stride()))
+            if lo < t.data_ptr() + (last + 1) * t.element_size():
+                raise ValueError("%s overlaps another argument" % name)
+
+
 def _clip_bounds(clip_eps):
     lo, hi = clip_eps if hasattr(clip_eps, "__len__") else (clip_eps, clip_eps)
     lo, hi = float(lo), float(hi)
@@ -630,6 +640,8 @@ def categorical_logprob_fwd(logits, index, out=None):
     dev = logits.device
     logp = torch.empty(B, dtype=torch.float32, device=dev) if out is None else out
     po = _rows(logp, B, dev, "logp")
+    if out is not None:
+        _apart(out, "logp", logits, index)
     if B == 0:
         return logp
     lib = _lib.load()
@@ -690,6 +702,8 @@ def categorical_ppo_fwd_bwd(logits, index, logp_old, adv, logp_ref=None, weight=
         logp, loss4 = out["logp"], out["loss4"]
         dlogits, pd, ldd = _logit_grad(out["dlogits"], logits)
         po, p4 = _rows(logp, B, dev, "logp"), _rows(loss4, 4, dev, "loss4")
+        read = (logits, index, logp_old, adv, logp_ref, weight, stats, dlogits)
+        _apart(logp, "logp", loss4, *read), _apart(loss4, "loss4", *read)
     out = {"logp": logp, "dlogits": dlogits, "loss4": loss4}
     if B == 0:
         loss4.zero_()
@@ -712,11 +726,13 @@ def policy_kl_loss(logp, logp_old, adv, logp_ref=None, weight=None, stats=None, 
     pl = _rows(logp, n, dev, "logp")
     lo, hi = _clip_bounds(clip_eps)
     head = _head_args(n, dev, logp_old, adv, logp_ref, weight, stats, kl_coef)
+    given = dlogp, loss4
     dlogp = torch.empty(n, dtype=torch.float32, device=dev) if dlogp is None else dlogp
     loss4 = torch.empty(4, dtype=torch.float32, device=dev) if loss4 is None else loss4
     pd, p4 = _rows(dlogp, n, dev, "dlogp"), _rows(loss4, 4, dev, "loss4")
-    if abs(pd - pl) < 4 * n:
-        raise ValueError("dlogp overlaps logp")
+    for t, name in zip(given, ("dlogp", "loss4")):
+        if t is not None:
+            _apart(t, name, logp, logp_old, adv, logp_ref, weight, stats, loss4 if t is dlogp else None)
     if n == 0:
         loss4.zero_()
         return dlogp, loss4

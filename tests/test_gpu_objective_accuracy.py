@@ -189,3 +189,35 @@ def test_preference_bounds_out_of_order(dev, T):
             assert bool(((d.double() - want).abs() <= U * want.abs() + 1e-9 / (len(bounds) // 2) + 1e-37).all()), bounds
             assert bool(((m.double() - margin).abs() <= U * margin.abs() + 1e-9).all()) and bool(torch.isfinite(l3).all())
         assert all(bool(t[:32].isnan().all()) and bool(t[-32:].isnan().all()) for t in held)
+
+
+def test_outputs_given_lie_apart_from_what_is_read(dev):
+    """an output on memory that other blocks still read (its own old log-probs, a piece of the weights) is refused before the launch"""
+    from pfpn_amd import kernels
+    x, k = torch.randn(8, 2, 5, device=dev), torch.zeros(8, 2, dtype=torch.int32, device=dev)
+    old, adv, ref, w = [torch.rand(8, device=dev) for _ in range(4)]
+    pool = torch.rand(64, device=dev)
+
+    def ppo(logp=None, loss4=None, dlogits=None, **kw):
+        out = {"logp": pool[:8] if logp is None else logp, "loss4": pool[8:12] if loss4 is None else loss4,
+               "dlogits": torch.zeros_like(x) if dlogits is None else dlogits}
+        a = dict(logp_old=old, adv=adv, logp_ref=ref, weight=w, kl_coef=0.1, out=out)
+        a.update(kw)
+        return kernels.categorical_ppo_fwd_bwd(x, k, a.pop("logp_old"), a.pop("adv"), **a)
+    want = kernels.categorical_ppo_fwd_bwd(x, k, old, adv, logp_ref=ref, weight=w, kl_coef=0.1)
+    got = ppo()
+    assert all(torch.equal(got[n], want[n]) for n in want)
+    for kw in (dict(logp=old), dict(logp=adv), dict(logp=ref), dict(logp=w), dict(logp=x.view(-1)[8:16]), dict(loss4=w[2:6]), dict(loss4=pool[6:10]),
+               dict(logp=pool[4:12], weight=pool[11:19]), dict(loss4=k.view(torch.float32).view(-1)[:4])):
+        with pytest.raises(ValueError, match="overlaps"):
+            ppo(**kw)
+    with pytest.raises(ValueError, match="overlaps"):
+        kernels.categorical_logprob_fwd(x, k, out=x.view(-1)[40:48])
+    assert torch.equal(kernels.categorical_logprob_fwd(x, k, out=pool[20:28]), kernels.categorical_logprob_fwd(x, k))
+    rows = dict(logp_ref=ref, weight=w, kl_coef=0.1)
+    want = kernels.policy_kl_loss(old, adv, ref, **rows)
+    got = kernels.policy_kl_loss(old, adv, ref, **rows, dlogp=pool[:8], loss4=pool[8:12])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for kw in (dict(dlogp=w), dict(dlogp=adv), dict(loss4=old[:4]), dict(dlogp=pool[:8], loss4=pool[7:11]), dict(dlogp=pool[4:12], stats=pool[11:15])):
+        with pytest.raises(ValueError, match="overlaps"):
+            kernels.policy_kl_loss(old, adv, ref, **dict(rows, **kw))
