@@ -278,10 +278,11 @@ __global__ __launch_bounds__(NT, E * IT > 32 ? 4 : 8) void k_cat_rows(CatArgs p)
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Long axes (N > 1024), rows that one block can hold (few very long ones: in pieces, below): a block owns a segment and keeps ALL of it in registers (H wide loads a
-// thread, raw), so the logits are read once whatever their length: one pass finds {m, s}, the gradient is formed from the registers.
-// For A = 1 (a token row) the loss head sits in between, run by one wave (three packs of eight wait in LDS meanwhile: its 64-bit
-// arithmetic would spill them).  1024 threads of at most 8 packs, two blocks a CU: one reads while the other writes.
+// Long axes (N > 1024), rows that one block can hold (few very long ones: in pieces, below): a block owns a segment and keeps ALL of
+// it in registers (H wide loads a thread, raw), so the logits are read once whatever their length: one pass finds {m, s}, the gradient
+// is formed from the registers.  For A = 1 (a token row) the loss head sits in between, run by one wave (of eight packs three wait in
+// LDS meanwhile: its 64-bit arithmetic would spill them).  64 to 1024 threads of four packs, 1024 of eight (two blocks a CU: one reads
+// while the other writes) or sixteen (one block a CU), the fewest that hold the row.
 // Bound: HBM.  6001 x 50021 bfloat16, a fifth of the rows without weight: 235 us = 4.6 TB/s (two kernels that read the logits twice:
 // 337 us); gradient of 2047 x 32001 float16: 55 us = 4.8 TB/s (86 us).  It was bound by instructions (23 an element) until the
 // exponent became one fma, the maxima packed and the join of the waves a lane each: 60 -> 55 us, 253 -> 235 us.

@@ -214,15 +214,6 @@ __device__ __forceinline__ float exp_below_exact(float x, float m) {
     return __builtin_amdgcn_exp2f(__builtin_fmaf(d, PFPN_LOG2E, d * 1.92596299e-8f));
 }
 
-// {max, sum exp(x - max)} of two parts of one axis joined; (-inf, 0) is the empty part
-__device__ __forceinline__ void join_softmax(float& m, float& s, float m2, float s2) {
-    const float mm = fmaxf(m, m2);
-    const float a = (m == mm) ? s : s * exp_below(m, mm);       // (m == mm also where both are -inf or +inf)
-    const float b = (m2 == mm) ? s2 : s2 * exp_below(m2, mm);
-    m = mm;
-    s = a + b;
-}
-
 // ---- a short axis (N <= 1024) over a group of G lanes: U packs of V consecutive categories a lane -------------------------------
 // Pack u of lane j is the segment's pack u G + j: a pack is one wide access from any alignment, the lanes' packs lie side by side.
 // The segment's last pack is moved down to end at N, so that every access is whole and inside the segment (V <= N): its first

@@ -826,10 +826,7 @@ static size_t bal_bytes(const BalArgs& p) {
 template <typename T, int G, int E, bool FULL>
 static void launch_bal_as(const BalArgs& p, hipStream_t st) {
     const int threads = (p.AT * p.RR * G + 63) / 64 * 64;
-    const size_t lds = ((size_t)p.RR + 1) * p.AT * p.N * 4;
-    if (lds > (64u << 10))
-        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&k_bal_stats<T, G, E, FULL>),
-                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    const size_t lds = ((size_t)p.RR + 1) * p.AT * p.N * 4;         // (RR AT N <= 576 E, AT N <= 4096: 52 KB at most)
     hipLaunchKernelGGL((k_bal_stats<T, G, E, FULL>), dim3(p.tiles * p.chunks), dim3(threads), lds, st, p);
     hipLaunchKernelGGL(k_bal_reduce, dim3((unsigned)bal_terms(p)), dim3(1024), 0, st, p);
     hipLaunchKernelGGL((k_bal_grad<T, G, E, FULL>), dim3(p.tiles * p.grad_chunks), dim3(threads), 0, st, p);
