@@ -812,9 +812,12 @@ static void bal_shape(BalArgs& p) {
     while (p.AT > 1 && p.AT * p.N > 4096) p.AT = (p.AT + 1) / 2;
     p.RR = groups / p.AT;
     p.tiles = (p.A + p.AT - 1) / p.AT;
-    // chunks of rows: two blocks a CU; four rows or more for a group of k_bal_stats (a chunk costs 8 A N bytes of slabs)
+    // chunks of rows: a block a CU; four rows or more for a group of k_bal_stats (a chunk costs 8 A N bytes of slabs), and 256 at most:
+    // a lane's 32-bit sum of as many equal weights, as a fresh policy has, is off by under 60 steps of 2^-24, of 3640 by 600 (the
+    // chunks are added in 64 bits)
     const long long most = ((long long)p.R + p.RR - 1) / p.RR, fill = (256 + p.tiles - 1) / p.tiles;
-    p.chunks = (int)((most + 3) / 4 < fill ? (most + 3) / 4 : fill);
+    const long long short_sums = (most + 255) / 256, wanted = fill > short_sums ? fill : short_sums;
+    p.chunks = (int)((most + 3) / 4 < wanted ? (most + 3) / 4 : wanted);
     p.grad_chunks = (int)(most < 4 * fill ? most : 4 * fill);
 }
 static size_t bal_terms(const BalArgs& p) { return ((size_t)p.A * p.N + BAL_COLS - 1) / BAL_COLS; }

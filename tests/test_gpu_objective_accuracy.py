@@ -48,6 +48,22 @@ def test_balance_gradient_of_nearly_equal_counts(dev, R, A, N, K, dtype):
         int((~ok).sum()), ok.numel(), float(((got[3].double() - grad).abs() / bound).masked_fill(ok, 0).max()))
 
 
+def test_balance_means_of_many_equal_rows(dev):
+    """2^24 rows of one fresh policy: equal weights, whose 32-bit sums round to one side"""
+    from pfpn_amd import kernels
+    gap = torch.tensor([0.125, 0.296875, 0.5, 0.703125, 1.296875, 1.5, 1.703125, 2.296875], device=dev)
+    row = torch.stack([gap, torch.zeros_like(gap)], -1).bfloat16()
+    x = row.expand(1 << 24, 8, 2).contiguous()
+    loss, counts, mean, _ = kernels.balance_loss(x)
+    want = torch.softmax(row.double(), -1)
+    assert counts[:, 0].tolist() == [1 << 24] * 8 and not counts[:, 1].any()
+    # a weight is off by its exponential, sum and quotient (12 u at these gaps); a lane adds 257 of them at most, a block its 18 rows
+    # of lanes; the chunks are added in 64 bits and rounded once
+    bound = (12 + 257 + 18 + 1) * U
+    assert float(((mean.double() - want).abs() / want).max()) <= bound
+    assert abs(float(loss) - float(2 / 8 * want[:, 0].sum())) <= bound * float(loss)
+
+
 # ---- clipped loss with a KL term: log-probs that lie far apart ------------------------------------------------------------------------
 def far_head(logp, old, adv, ref, w, eps, c, err=0.0):
     """-> dlogp, its bound, loss4 and its bound, in 64 bits.  The kernels' differences, exponentials and products are 64-bit; the series of
