@@ -4,7 +4,8 @@ import math
 import pytest
 import torch
 
-from _objectives import U, balance, gradient, logprob, preference, rounded, segment_bound, softmax
+from _objectives import U, balance, gradient, head, logprob, preference, rounded, segment_bound, softmax
+from test_gpu_objectives import SHAPES, close, make_logits, objective
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -237,3 +238,25 @@ def test_outputs_given_lie_apart_from_what_is_read(dev):
     for kw in (dict(dlogp=w), dict(dlogp=adv), dict(loss4=old[:4]), dict(dlogp=pool[:8], loss4=pool[7:11]), dict(dlogp=pool[4:12], stats=pool[11:15])):
         with pytest.raises(ValueError, match="overlaps"):
             kernels.policy_kl_loss(old, adv, ref, **dict(rows, **kw))
+
+
+# ---- float16 logits in the clipped loss -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("shape", SHAPES)
+def test_policy_loss_from_float16_logits(dev, shape):
+    """the shapes of the float32 and bfloat16 test, under its bounds; weights of about one, so that gradients stay above float16's
+    smallest step"""
+    from pfpn_amd import kernels
+    B, A, N = shape
+    x, k, g = make_logits(dev, B, A, N, torch.float16, pad=N % 3, seed=2 * N + A, closed=0.05 if N % 2 else 0.0)
+    logp, err = logprob(x, k)
+    old, adv, ref, w = objective(dev, logp, g, True)
+    w[0] = 0.7
+    for ref_, c, stats in ((ref, 0.05, None), (None, 0.0, torch.tensor([0.1, 1.7, -1.0, 1.5], device=dev))):
+        got = kernels.categorical_ppo_fwd_bwd(x, k.int(), old, adv, logp_ref=ref_, weight=w, stats=stats, clip_eps=(0.2, 0.3), kl_coef=c)
+        dlogp, derr, loss4 = head(logp, old, adv, ref_, w, 0.2, 0.3, c, stats, err)
+        close(got["logp"], torch.where(w != 0, logp, torch.zeros_like(logp)), err, "logp")
+        wg, bg = gradient(x, k, dlogp, derr)
+        assert got["dlogits"].dtype == torch.float16
+        close(got["dlogits"], wg, rounded(wg, bg, torch.float16), "dlogits")
+        lsum = derr.sum() + U * loss4.abs().sum() + 1e-30
+        close(got["loss4"], loss4, torch.full((4,), float(lsum), device=dev, dtype=torch.float64), "loss4")
