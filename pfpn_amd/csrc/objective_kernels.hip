@@ -95,31 +95,40 @@ __device__ __forceinline__ void outside_zero(const PrefArgs& p, long long id, lo
     for (long long t = last + id; t < p.T; t += n) p.dlogp[t] = 0.f;
 }
 
-// loss of one pair -> d loss / d delta (of the mean); fills its terms[3] and margin when `write`
-__device__ __forceinline__ double pair_head(const PrefArgs& p, int pair, double delta, bool write, double* terms) {
+// A pair's head, in 64 bits: e sigma(m) - (1 - e) sigma(-m) cancels near its zero, and an exponential in 32 is off by |m| 2^-24 of
+// itself.  Both halves of it from ONE exponential of -|m|; log sigma(m) = -softplus(-m).
+// d loss / d delta, of the mean over the pairs; z = e^-|margin|
+__device__ __forceinline__ double pair_slope(const PrefArgs& p, double delta, double& z) {
+    z = 0.0;
+    if (p.kind) return 2.0 * (delta - 0.5 / p.beta) / (double)p.P;
+    const double m = p.beta * delta, e = p.smoothing;
+    z = exp(-fabs(m));
+    const double near = 1.0 / (1.0 + z), far = z * near;
+    return p.beta * (m >= 0 ? e * near - (1.0 - e) * far : e * far - (1.0 - e) * near) / (double)p.P;
+}
+// log(1 + z), z in [0, 1]: 2 artanh(z / (2 + z)), whose argument is 1/3 at most: the first term left out is under 2^-40 of the sum
+__device__ __forceinline__ double log_one_plus(double z) {
+    const double s = z / (2.0 + z), q = s * s;
+    double t = 1.0 / 23.0;
+#pragma unroll
+    for (int k = 21; k > 0; k -= 2) t = __builtin_fma(t, q, 1.0 / k);
+    return 2.0 * s * t;
+}
+// {loss, margin > 0, margin}, and the pair's margin
+__device__ __forceinline__ void pair_terms(const PrefArgs& p, int pair, double delta, double z, double* terms) {
     const double m = p.beta * delta;
-    double loss = 0.0, slope;
+    double loss;
     if (p.kind == 0) {
-        // log sigma(m) = -softplus(-m); both halves from ONE exponential of -|m|.  In 64 bits: e sigma(m) - (1 - e) sigma(-m) cancels
-        // near its zero, and an exponential in 32 is off by |m| 2^-24 of itself
-        const double e = p.smoothing, am = fabs(m), z = exp(-am), near = 1.0 / (1.0 + z), far = z * near;
-        slope = p.beta * (m >= 0 ? e * near - (1.0 - e) * far : e * far - (1.0 - e) * near);
-        if (write) {
-            const double l = log1p(z);
-            loss = (1.0 - e) * (l + (m < 0 ? am : 0.0)) + (e > 0 ? e * (l + (m > 0 ? am : 0.0)) : 0.0);   // (infinite margin: 0, not 0 * inf)
-        }
+        const double e = p.smoothing, am = fabs(m), l = log_one_plus(z);
+        loss = (1.0 - e) * (l + (m < 0 ? am : 0.0)) + (e > 0 ? e * (l + (m > 0 ? am : 0.0)) : 0.0);     // (infinite margin: 0, not 0 * inf)
     } else {
         const double u = delta - 0.5 / p.beta;
         loss = u * u;
-        slope = 2.0 * u;
     }
-    if (write) {
-        p.margin[pair] = (float)m;
-        terms[0] = loss;
-        terms[1] = m > 0 ? 1.0 : 0.0;
-        terms[2] = m;
-    }
-    return slope / (double)p.P;
+    p.margin[pair] = (float)m;
+    terms[0] = loss;
+    terms[1] = m > 0 ? 1.0 : 0.0;
+    terms[2] = m;
 }
 
 // Few steps: ONE block, a wave per pair in turn (a launch costs more than the work).
@@ -128,14 +137,27 @@ __device__ __forceinline__ double pair_head(const PrefArgs& p, int pair, double 
 // which are too few to fill the chip)
 constexpr int PREF_SHORT = 1024, PREF_SMALL_P = 128, PREF_SMALL_T = 16384;
 __global__ __launch_bounds__(1024) void k_pref_small(PrefArgs p, float* __restrict__ loss3) {
-    __shared__ double terms[PREF_SMALL_P * 3];
+    __shared__ double terms[PREF_SMALL_P * 3], gap[PREF_SMALL_P];
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
     for (int pair = wid; pair < p.P; pair += 16) {
         const PairRows r = rows_of_pair(p, pair);
         const double delta = group_sum<64>(span_sum(p, r.lo, r.hi, r.mid, lane, 64));
-        span_grad(p, r.lo, r.hi, r.mid, lane, 64, pair_head(p, pair, delta, lane == 0, terms + pair * 3));
+        if (lane == 0) gap[pair] = delta;
     }
     outside_zero(p, threadIdx.x, 1024);
+    __syncthreads();
+    // (a thread a pair: a wave that runs its pairs' heads in turn takes 1 us for each)
+    double delta = 0.0, z = 0.0;
+    if ((int)threadIdx.x < p.P) {
+        delta = gap[threadIdx.x];
+        gap[threadIdx.x] = pair_slope(p, delta, z);
+    }
+    __syncthreads();
+    for (int pair = wid; pair < p.P; pair += 16) {
+        const PairRows r = rows_of_pair(p, pair);
+        span_grad(p, r.lo, r.hi, r.mid, lane, 64, gap[pair]);
+    }
+    if ((int)threadIdx.x < p.P) pair_terms(p, threadIdx.x, delta, z, terms + threadIdx.x * 3);
     __syncthreads();
     if (wid < 3) {
         double t = 0.0;
@@ -198,7 +220,8 @@ __global__ __launch_bounds__(256) void k_pref_pairs(PrefArgs p) {
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
         const double delta = ((red[0] + red[1]) + red[2]) + red[3];
-        const double g = pair_head(p, blockIdx.x, delta, threadIdx.x == 0, p.terms + (size_t)blockIdx.x * 3);
+        double z;
+        const double g = pair_slope(p, delta, z);
         float* d = p.dlogp + r.lo;
 #pragma unroll
         for (int h = 0; h < H; ++h) {
@@ -210,13 +233,16 @@ __global__ __launch_bounds__(256) void k_pref_pairs(PrefArgs p) {
             }
         }
         if (tail < steps) d[tail] = step_grad(tail >= mid ? -g : g, wl);
+        if (threadIdx.x == 0) pair_terms(p, blockIdx.x, delta, z, p.terms + (size_t)blockIdx.x * 3);
         return;
     }
     const double v = group_sum<64>(span_sum(p, r.lo, r.hi, r.mid, threadIdx.x, 256));
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     const double delta = ((red[0] + red[1]) + red[2]) + red[3];
-    span_grad(p, r.lo, r.hi, r.mid, threadIdx.x, 256, pair_head(p, blockIdx.x, delta, threadIdx.x == 0, p.terms + (size_t)blockIdx.x * 3));
+    double z;
+    span_grad(p, r.lo, r.hi, r.mid, threadIdx.x, 256, pair_slope(p, delta, z));
+    if (threadIdx.x == 0) pair_terms(p, blockIdx.x, delta, z, p.terms + (size_t)blockIdx.x * 3);
 }
 
 // Many short pairs: G lanes a pair, no barrier between sums and gradients; a block leaves the sum of its pairs' terms (fixed order).
@@ -237,10 +263,15 @@ __global__ __launch_bounds__(256) void k_pref_groups(PrefArgs p, int blocks) {
         double delta = on ? span_sum(p, r.lo, r.hi, r.mid, lane, G) : 0.0;
         delta = group_sum<G>(delta);
         if (on) {
-            double own[3];
-            const double g = pair_head(p, pair, delta, lane == 0, own);
-            span_grad(p, r.lo, r.hi, r.mid, lane, G, g);
-            if (lane == 0) { t[0] += own[0]; t[1] += own[1]; t[2] += own[2]; }
+            double z;
+            span_grad(p, r.lo, r.hi, r.mid, lane, G, pair_slope(p, delta, z));
+            if (lane == 0) {
+                double own[3];
+                pair_terms(p, pair, delta, z, own);
+                t[0] += own[0];
+                t[1] += own[1];
+                t[2] += own[2];
+            }
         }
     }
     if (lane == 0) {
@@ -279,11 +310,13 @@ __global__ __launch_bounds__(256) void k_pref_grad(PrefArgs p) {
     const double* sums = p.sums + (size_t)pair * p.splits;
     double d = 0.0;
     for (int i = lane; i < p.splits; i += 64) d += sums[i];
-    const double g = pair_head(p, pair, group_sum<64>(d), threadIdx.x == 0 && part == 0, p.terms + (size_t)pair * 3);
+    const double delta = group_sum<64>(d);
     const PairRows r = rows_of_pair(p, pair);
     long long lo, hi;
     piece_of_pair(p, r, part, lo, hi);
-    span_grad(p, lo, hi, r.mid, threadIdx.x, 256, g);
+    double z;
+    span_grad(p, lo, hi, r.mid, threadIdx.x, 256, pair_slope(p, delta, z));
+    if (threadIdx.x == 0 && part == 0) pair_terms(p, pair, delta, z, p.terms + (size_t)pair * 3);
 }
 
 __global__ __launch_bounds__(FINISH_NT) void k_pref_finish(const double* __restrict__ terms, size_t n, int step, int P, float* __restrict__ loss3) {
