@@ -131,11 +131,15 @@ __device__ __forceinline__ void pair_terms(const PrefArgs& p, int pair, double d
     terms[2] = m;
 }
 
-// Few steps: ONE block, a wave per pair in turn (a launch costs more than the work).
-// (PREF_SHORT: up to so many steps a pair, many pairs go by lanes, not by blocks.  20000 pairs of 100: 44 us by blocks, 25 us by waves,
-// 12 us by 16 lanes with the blocks' terms summed; 3000 of 1000: 13.9 / 13.0 us; but 400 of 1000: 7.3 us by blocks, 8.5 us by waves,
-// which are too few to fill the chip)
-constexpr int PREF_SHORT = 1024, PREF_SMALL_P = 128, PREF_SMALL_T = 16384;
+// Few steps: ONE block, a wave per pair in turn.  It saves a launch, 2 us of a call's 14 on the host, as long as its own time stays under
+// the call's (us by one block / by the general forms, in a graph): 24 pairs of 100 steps 4.6 / 4.6, 16 of 1000 6.6 / 4.7, 64 of 256
+// 9.0 / 4.7, all in calls of 12 / 14; 1 of 2000 6.1 / 4.6.  Beyond, it costs more: 128 of 64 15.8 / 5.1, 1 of 16384 32 / 12.
+constexpr int PREF_SMALL_P = 64, PREF_SMALL_T = 16384, PREF_SMALL_MEAN = 2048;
+// PREF_SHORT: up to so many steps a pair, many pairs go by lanes (16 up to 128 steps, else 64), not by blocks, with the blocks' terms
+// summed: from three times as many pairs as steps on there are lanes enough to fill the chip.  By lanes / by blocks: 20000 pairs of 20
+// 11.5 / 35, of 100 13.1 / 38, of 300 31 / 42; 3000 of 300 10.6 / 12.5, of 1000 14.4 / 15.2; 600 of 300 8.6 / 8.8, of 600 9.1 / 9.1;
+// fewer: 600 of 1000 9.6 / 9.2, 1500 of 1000 11.4 / 10.9, 200 of 1000 9.0 / 8.0.
+constexpr int PREF_SHORT = 1024;
 __global__ __launch_bounds__(1024) void k_pref_small(PrefArgs p, float* __restrict__ loss3) {
     __shared__ double terms[PREF_SMALL_P * 3], gap[PREF_SMALL_P];
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
@@ -930,7 +934,7 @@ int pfpn_preference_loss(const float* logp, const float* logp_ref, const float* 
     hipStream_t st = (hipStream_t)stream;
     const unsigned blocks = (unsigned)P * (unsigned)p.splits;
     const unsigned outside = (unsigned)(T / 4096 + 1 < 64 ? T / 4096 + 1 : 64);
-    if (P <= PREF_SMALL_P && T <= PREF_SMALL_T) {
+    if (P <= PREF_SMALL_P && T <= PREF_SMALL_T && T / P <= PREF_SMALL_MEAN) {
         hipLaunchKernelGGL(k_pref_small, dim3(1), dim3(1024), 0, st, p, loss3);
         PFPN_CHECK_LAUNCH();
         return PFPN_OK;
