@@ -843,12 +843,22 @@ static int group_width(int N) {
     return N <= 4 ? 4 : N <= 8 ? 2 : N <= 24 ? 4 : N <= 64 ? 8 : N <= 96 ? 16 : N <= 128 ? 8 : N <= 256 ? 32 : 64;
 }
 
-static void bal_shape(BalArgs& p) {
-    const int G = group_width(p.N), groups = BAL_NT / 64 * 64 / G;
+// choices and rows side by side in a block of up to `threads`; -> its time for a row of all choices: the tiles of choices over the rows
+// that a block takes at once, by the waves of its fullest SIMD (k_bal_stats is bound by issue, one block a CU)
+static double bal_block(BalArgs& p, int threads) {
+    const int G = group_width(p.N), groups = threads / G;
     p.AT = p.A < groups ? p.A : groups;
     while (p.AT > 1 && p.AT * p.N > 4096) p.AT = (p.AT + 1) / 2;
     p.RR = groups / p.AT;
     p.tiles = (p.A + p.AT - 1) / p.AT;
+    return (double)p.tiles / p.RR * ((p.AT * p.RR * G + 255) / 256);
+}
+static void bal_shape(BalArgs& p) {
+    // Eight waves, two a SIMD, or nine where they take another row of choices or a tile less, by that time.  Loss, eight / nine waves
+    // (us): 262147 x 128 bfloat16 top 8 67 / 78, 8192 x 128 x 256 656 / 901, 200000 x 300 274 / 315, 20000 x 17 x 24 28.7 / 30.0;
+    // 4096 x 36 x 35 27.9 / 24.7, 3000 x 130 x 40 53.8 / 48.6, 9000 x 3 x 1000 78 / 75.
+    const double eight = bal_block(p, 512);
+    if (bal_block(p, BAL_NT) > eight) bal_block(p, 512);
     // chunks of rows: a block a CU; four rows or more for a group of k_bal_stats (a chunk costs 8 A N bytes of slabs), and 256 at most:
     // a lane's 32-bit sum of as many equal weights, as a fresh policy has, is off by under 60 steps of 2^-24, of 3640 by 600 (the
     // chunks are added in 64 bits)
