@@ -100,18 +100,49 @@ int cat_splits(int B, int A, int N) {
     return (int)(s < 1 ? 1 : s > CAT_MAX_SPLITS ? CAT_MAX_SPLITS : s);
 }
 
+// One launch takes MAX_BLOCKS blocks: more rows go in turns.  Their loss terms line up in the workspace; what else a turn keeps there
+// lies behind its own terms, and is done with before the next turn's are written.
+static size_t rows_of_a_launch(const CatArgs& p, size_t size) {
+    if (p.N > CAT_SHORT_N) return MAX_BLOCKS / p.A;                 // a block a segment (many rows: one piece each)
+    // (a block of a large batch takes sixteen segments in whole rows, or more, where they span less than 2^31 bytes)
+    const size_t widest = (size_t)(p.ld > p.ldd ? p.ld : p.ldd) * size;
+    return p.A < 16 && widest < (1ull << 31) / 16 ? MAX_BLOCKS * (16 / p.A) : MAX_BLOCKS;
+}
+
 template <int MODE>
 static int run_typed(CatArgs p, int dtype, void* ws, size_t ws_bytes, float* loss4, void* stream) {
     hipStream_t st = (hipStream_t)stream;
-    p.loss4 = loss4;
-    size_t nparts = 0;
-    const int rc = dtype == DT_F32 ? run_cat<float, MODE>(p, ws, ws_bytes, &nparts, st)
-                 : dtype == DT_BF16 ? run_cat<bf16_t, MODE>(p, ws, ws_bytes, &nparts, st)
-                                    : run_cat<f16_t, MODE>(p, ws, ws_bytes, &nparts, st);
-    if (rc != PFPN_OK || MODE != CAT_PPO || nparts == 0) return rc;
+    const size_t size = dtype == DT_F32 ? 4 : 2, rows = p.B, most = rows_of_a_launch(p, size);
+    size_t total = 0;
+    for (size_t r = 0; r < rows; r += most) {
+        CatArgs q = p;
+        q.B = (int)(rows - r < most ? rows - r : most);
+        q.logits = static_cast<const char*>(p.logits) + r * p.ld * size;
+        q.index = static_cast<const int*>(p.index) + (r * p.A << p.index64);
+        if (p.logp) q.logp += r;
+        if (p.dlogp) q.dlogp += r;
+        if (p.dlogits) q.dlogits = static_cast<char*>(p.dlogits) + r * p.ldd * size;
+        if (MODE == CAT_PPO) {
+            q.head.logp_old += r;
+            q.head.adv += r;
+            if (p.head.logp_ref) q.head.logp_ref += r;
+            if (p.head.weight) q.head.weight += r;
+        }
+        q.loss4 = rows <= most ? loss4 : nullptr;
+        const size_t used = total * 3 * sizeof(double);
+        void* at = ws ? static_cast<char*>(ws) + used : nullptr;
+        const size_t left = ws_bytes > used ? ws_bytes - used : 0;
+        size_t nparts = 0;
+        const int rc = dtype == DT_F32 ? run_cat<float, MODE>(q, at, left, &nparts, st)
+                     : dtype == DT_BF16 ? run_cat<bf16_t, MODE>(q, at, left, &nparts, st)
+                                        : run_cat<f16_t, MODE>(q, at, left, &nparts, st);
+        if (rc != PFPN_OK) return rc;
+        if (MODE == CAT_PPO) total += nparts;
+    }
+    if (MODE != CAT_PPO || total == 0) return PFPN_OK;
     double* part = static_cast<double*>(ws);
-    const int step = fold_terms(part, nparts, st);
-    hipLaunchKernelGGL(k_policy_finish, dim3(1), dim3(FINISH_NT), 0, st, (const double*)part, nparts, step, p.head.kl_coef, loss4);
+    const int step = fold_terms(part, total, st);
+    hipLaunchKernelGGL(k_policy_finish, dim3(1), dim3(FINISH_NT), 0, st, (const double*)part, total, step, p.head.kl_coef, loss4);
     PFPN_CHECK_LAUNCH();
     return PFPN_OK;
 }

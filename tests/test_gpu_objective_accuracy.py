@@ -260,3 +260,36 @@ def test_policy_loss_from_float16_logits(dev, shape):
         close(got["dlogits"], wg, rounded(wg, bg, torch.float16), "dlogits")
         lsum = derr.sum() + U * loss4.abs().sum() + 1e-30
         close(got["loss4"], loss4, torch.full((4,), float(lsum), device=dev, dtype=torch.float64), "loss4")
+
+
+# ---- more rows than one launch has blocks -----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("shape", [((1 << 22) + 5, 1, 1025), ((1 << 22) + 2, 20, 3), ((1 << 21) + 3, 2, 1030)])
+def test_more_rows_than_a_launch_has_blocks(dev, shape):
+    """the rows on both sides of where a launch ends against the same rows alone (row weights small powers of two: the same bits), the
+    loss against the sum over parts"""
+    from pfpn_amd import kernels
+    B, A, N = shape
+    g = torch.Generator(device=dev)
+    g.manual_seed(N)
+    x = torch.empty(B, A, N, dtype=torch.float16, device=dev)
+    for lo in range(0, B, 1 << 18):
+        x[lo:lo + (1 << 18)].normal_(generator=g)
+    k = torch.randint(0, N, (B, A), device=dev, generator=g)
+    adv, w = torch.randn(B, device=dev, generator=g), torch.full((B,), 2.0 ** -4, device=dev)
+    logp = kernels.categorical_logprob_fwd(x, k)
+    old = logp + 0.1 * torch.randn(B, device=dev, generator=g)
+    got = kernels.categorical_ppo_fwd_bwd(x, k, old, adv, logp_ref=logp, weight=w, kl_coef=0.1)
+    d = kernels.categorical_logprob_bwd(x, k, adv)
+    edge = ((1 << 22) - 1) // (1 if N <= 1024 else A)
+    for lo in (0, edge - 30, B - 40):
+        part = slice(lo, lo + 40)
+        assert torch.equal(logp[part], kernels.categorical_logprob_fwd(x[part], k[part]))
+        assert torch.equal(d[part], kernels.categorical_logprob_bwd(x[part], k[part], adv[part]))
+        alone = kernels.categorical_ppo_fwd_bwd(x[part], k[part], old[part], adv[part], logp_ref=logp[part], weight=w[part], kl_coef=0.1)
+        assert torch.equal(got["dlogits"][part], alone["dlogits"]) and torch.equal(got["logp"][part], alone["logp"])
+    half = B // 2
+    parts = [kernels.categorical_ppo_fwd_bwd(x[s], k[s], old[s], adv[s], logp_ref=logp[s], weight=w[s], kl_coef=0.1)["loss4"].double()
+             for s in (slice(0, half), slice(half, B))]
+    total = parts[0] + parts[1]
+    scale = 2.0 ** -4 * torch.tensor([2.0, 2.0, 1.0, 1.0], device=dev, dtype=torch.float64) * B
+    assert bool(((got["loss4"].double() - total).abs() <= U * (parts[0].abs() + parts[1].abs() + total.abs()) + 1e-14 * scale).all())
