@@ -225,8 +225,9 @@ int pfpn_resample(float* loc, float* logstd, float* bias, float* weight, int H,
  * `row_stride` elements (>= A*N: a padded row), the [A, N] part of a row dense; any alignment of the element type.  A = 1: one
  * choice of N per row (a token of a vocabulary).  A <= 4096, N <= 2^30.  `index` [B, A]: int32, or int64 with index64 != 0; an
  * index outside [0, N) takes its choice out of the row (log-prob 0, zero gradient).  A logit of -inf closes a category; a segment
- * with every category closed has log-prob -inf and a zero gradient.  Gradients have the logits' type, one rounding from 32 bits;
- * dlogits must not overlap logits.  Workspaces need no initialisation; results are bitwise reproducible. */
+ * with every category closed has log-prob -inf and a zero gradient.  Gradients have the logits' type, one rounding from 32 bits.
+ * Outputs must not overlap inputs, nor each other.  Workspaces (16-byte aligned) need no initialisation; results are bitwise
+ * reproducible. */
 size_t pfpn_categorical_workspace_bytes(int B, int A, int N);
 /* logp[b] = sum_a log softmax(logits[b,a,:])[index[b,a]] -- the log-prob of the categories a policy drew (the index draw:
  * reference networks/utils.py:187-194). */
@@ -242,7 +243,9 @@ int pfpn_categorical_logprob_bwd(const void* logits, int dtype, long long row_st
  *   a = clip((adv - mean) rstd) (adv_stats NULL: adv itself), r = exp(logp - logp_old), d = logp_ref - logp,
  *   loss = sum_b w_b (-min(r a, clip(r, 1 - clip_eps_low, 1 + clip_eps_high) a) + kl_coef (exp(d) - 1 - d)).
  * logp_ref optional (NULL: no KL term, kl_coef must be 0); weight [B] optional (NULL: 1/B each) -- a row of weight 0 does not count
- * whatever it holds, its logp and gradient are 0.  An impossible choice (logp -inf) makes the KL term infinite.  loss4 = {loss, sum w policy term, sum w kl, sum of w where the clip binds}. */
+ * whatever it holds, its logp and gradient are 0.  r, exp(d) and their products are 64-bit; a row with a = 0 has no policy term
+ * however large its ratio.  An impossible choice (logp -inf) makes the KL term infinite.
+ * loss4 = {loss, sum w policy term, sum w kl, sum of w where the clip binds}. */
 int pfpn_categorical_ppo_fwd_bwd(const void* logits, int dtype, long long row_stride, const void* index, int index64,
                                  const float* logp_old, const float* adv, const float* logp_ref, const float* weight,
                                  const float* adv_stats, int B, int A, int N, double clip_eps_low, double clip_eps_high,
@@ -254,8 +257,8 @@ int pfpn_policy_kl_loss(const float* logp, const float* logp_old, const float* a
                         const float* weight, const float* adv_stats, long long n, double clip_eps_low, double clip_eps_high,
                         double kl_coef, float* dlogp, float* loss4, void* workspace, size_t workspace_bytes, void* stream);
 /* Loss over P pairs of compared segments (paired log ratios; offsets as pfpn_gae's: segment s = rows [offsets[s],
- * offsets[s+1]) of the T log-probs, DEVICE int64 [2P+1], ascending; clamped to [0, T] and to
- * ascend within a pair; pair p prefers segment 2p to 2p+1):
+ * offsets[s+1]) of the T log-probs, DEVICE int64 [2P+1], ascending (clamped to [0, T] and to ascend within a pair); pair p prefers
+ * segment 2p to 2p+1):
  *   S_s = sum_t w_t (logp_t - logp_ref_t), delta = S_2p - S_2p+1, margin = beta delta,
  *   kind 0: -(1 - e) log sigma(margin) - e log sigma(-margin) (e = label_smoothing); kind 1: (delta - 1 / (2 beta))^2; mean over P.
  * logp_ref, weight optional; a step of weight 0 is skipped whatever it holds.  dlogp [T] is written for every row (0 outside all
@@ -267,8 +270,10 @@ int pfpn_preference_loss(const float* logp, const float* logp_ref, const float* 
 /* Balance loss over the categories of each choice, with counts (keeps particles from dying out, as pfpn_active_stats measures
  * them: reference a2c.py:346-365).  Over the V rows that mask (uint8 [R], optional) leaves: counts[a,n] = rows whose topk largest
  * logits hold n (equal ones: lowest index first; -inf never), f = counts / (topk V), mean_prob = mean softmax,
- *   loss = coef N / A sum_{a,n} f mean_prob (>= coef, = coef when balanced), dlogits (+)= coef N / (A V) p_n (f_n - sum_m f_m p_m).
- * Masked rows do not count whatever they hold, their gradient is 0 (accumulate: left alone).  N <= 1024, A <= 4096, topk <= min(N, 64). */
+ *   loss = coef N / A sum_{a,n} f mean_prob (coef where f or mean_prob is uniform; no lower bound: where the largest weight of most
+ *   rows is a narrow one it can be less), dlogits (+)= coef N / (A V) p_n (f_n - sum_m f_m p_m).
+ * Masked rows do not count whatever they hold, their gradient is 0 (accumulate: left alone).  R <= 2^30, N <= 1024, A <= 4096,
+ * topk <= min(N, 64). */
 size_t pfpn_balance_workspace_bytes(int R, int A, int N);
 int pfpn_balance_loss(const void* logits, int dtype, long long row_stride, const uint8_t* mask, int R, int A, int N, int topk,
                       double coef, int accumulate, float* loss, int32_t* counts, float* mean_prob, void* dlogits,

@@ -793,11 +793,11 @@ def balance_loss(logits, topk=1, coef=1.0, mask=None, dlogits=None, out=None):
     """Balance loss over the N categories of each choice: logits [R,A,N] (or [R,N]); a row counts for its `topk` largest
     logits (equal ones: the lowest index first; -inf never); mask [R] bool: rows that count.  `dlogits` given: the gradient
     is added to it.  `out` = (loss, counts, mean_prob): tensors to write into.
-    -> loss [1] (= coef when balanced), counts [A,N] int32, mean_prob [A,N], dlogits."""
+    -> loss [1] (coef where all shares or all mean weights are equal), counts [A,N] int32, mean_prob [A,N], dlogits."""
     pl, dt, ld, R, A, N = _logit_rows(logits)
     dev, topk = logits.device, int(topk)
-    if N > 1024 or not 1 <= topk <= min(N, 64):
-        raise ValueError("balance_loss: N = %d, topk = %d: N <= 1024 and 1 <= topk <= min(N, 64)" % (N, topk))
+    if N > 1024 or R > 1 << 30 or not 1 <= topk <= min(N, 64):
+        raise ValueError("balance_loss: %d rows, N = %d, topk = %d: at most 2^30 rows, N <= 1024 and 1 <= topk <= min(N, 64)" % (R, N, topk))
     pm = None
     if mask is not None:
         if not (isinstance(mask, torch.Tensor) and mask.is_cuda and mask.dtype in (torch.bool, torch.uint8) and

@@ -65,6 +65,18 @@ def test_balance_means_of_many_equal_rows(dev):
     assert abs(float(loss) - float(2 / 8 * want[:, 0].sum())) <= bound * float(loss)
 
 
+def test_balance_loss_can_be_less_than_its_coefficient(dev):
+    """three rows of five at weights (0.51, 0.49), two at (0, 1): shares (0.6, 0.4) of means (0.306, 0.694), 2 (0.6 x 0.306 + 0.4 x 0.694)"""
+    from pfpn_amd import kernels
+    x = torch.tensor([[math.log(0.51), math.log(0.49)]] * 3 + [[-math.inf, 0.0]] * 2, device=dev).unsqueeze(1)
+    loss, counts, mean, _ = kernels.balance_loss(x, coef=0.5)
+    assert counts.tolist() == [[3, 2]] and abs(float(loss) - 0.5 * 0.9224) < 1e-6
+    # equal shares, or equal mean weights: the coefficient
+    assert abs(float(kernels.balance_loss(x[[0, 3]], coef=0.5)[0]) - 0.5) < 1e-6
+    even = torch.tensor([[0.9, 0.1], [0.45, 0.55], [0.15, 0.85]], device=dev).log().unsqueeze(1)
+    assert abs(float(kernels.balance_loss(even, coef=0.5)[0]) - 0.5) < 1e-6
+
+
 # ---- clipped loss with a KL term: log-probs that lie far apart ------------------------------------------------------------------------
 def far_head(logp, old, adv, ref, w, eps, c, err=0.0):
     """-> dlogp, its bound, loss4 and its bound, in 64 bits.  The kernels' differences, exponentials and products are 64-bit; the series of
