@@ -103,6 +103,8 @@ class ParticleFilteringA2CNetwork(A2CNetwork):
         # preference_beta / _smoothing: train_preference's loss
         self.balance_beta = balance_beta
         self.preference_beta, self.preference_smoothing = float(preference_beta), float(preference_smoothing)
+        if kwargs.get("kl_coef"):
+            raise NotImplementedError("kl_coef belongs to the clipped-PPO network")
         if balance_beta and self.particles > 1024:
             raise ValueError("balance_beta: at most 1024 particles")
         if not 0.0 < self.preference_beta < float("inf") or not 0.0 <= self.preference_smoothing <= 0.5:

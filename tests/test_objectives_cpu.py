@@ -120,3 +120,14 @@ def test_networks_without_a_value_trunk_refuse_preference_steps(cls):
     for call in (net.compute_preference_gradients, lambda *a: net.train_preference(None, None, [], *a)):
         with pytest.raises(NotImplementedError, match="train_preference"):
             call(torch.zeros(4, 5), torch.zeros(4, 2), torch.tensor([0, 2, 4]))
+
+
+@pytest.mark.parametrize("cls", ["ParticleFilteringA2CNetwork", "ParticleFilteringVTraceNetwork", "ParticleFilteringSACNetwork",
+                                 "ParticleFilteringDDPGNetwork"])
+def test_kl_coef_is_not_taken_silently(cls):
+    from pfpn_amd import networks
+    base = dict(trainable=True, state_shape=[5], action_shape=[2], action_lower_bound=[-1, -1], action_upper_bound=[1, 1],
+                common_net_shape=[], critic_net_shape=[8], actor_net_shape=[8])
+    with pytest.raises(NotImplementedError, match="kl_coef"):
+        getattr(networks, cls)(**base, kl_coef=0.1)
+    getattr(networks, cls)(**base, kl_coef=0.0)
