@@ -6,6 +6,7 @@ dispatch cost is comparable to the device time, so the whole device part of the 
 Host-side bookkeeping (global_step, the resample tick every `resample_interval` steps) stays outside
 the graph: the resample kernels run eagerly between replays.
 """
+import contextlib
 import gc
 import os
 import sys
@@ -38,6 +39,20 @@ def release_captured_collectives():
     if torch.cuda.is_available():
         torch.cuda.synchronize()
     return n
+
+
+@contextlib.contextmanager
+def capturing(graph, stream, **mode):
+    """torch.cuda.graph(), with the collector paused: a cycle that is collected in between may own an older network's graph, whose
+    destruction the runtime refuses during a capture -- an exception in a destructor, which ends the process."""
+    was_on = gc.isenabled()
+    gc.disable()
+    try:
+        with torch.cuda.graph(graph, stream=stream, **mode):
+            yield
+    finally:
+        if was_on:
+            gc.enable()
 
 
 def _capture_mode(force=False):
@@ -291,7 +306,7 @@ class GraphedLearnerStep(object):
         # the default -- global -- mode a query from ANOTHER thread invalidates this thread's capture: the "operation failed
         # due to a previous error during capture" that one full-suite run in seven died of in round 4)
         mode = _capture_mode(self.in_graph_exchange)
-        with torch.cuda.graph(self.graph, stream=s, **mode):      # same stream as the warm-up: per-stream workspaces exist
+        with capturing(self.graph, s, **mode):      # same stream as the warm-up: per-stream workspaces exist
             if gather_from is not None:
                 kernels.gather_columns(list(gather_from[0]), list(self.input_sets[0]), gather_from[1][0])
             for k in range(self.K):
@@ -321,7 +336,7 @@ class GraphedLearnerStep(object):
                     gather_from[2][k].copy_(self.loss3)
         if self.split:
             self.graph_post = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(self.graph_post, stream=s, **mode):
+            with capturing(self.graph_post, s, **mode):
                 optimizer.post_reduce(net)
         # capture does not execute; state is untouched
         # True: EVERY captured step's optimiser launch took the noise rider, so only the FIRST replay needs a draw from outside.
@@ -449,7 +464,7 @@ class GraphedRollout(object):
         for t, sv in zip(stats, saved):
             t.copy_(sv)
         self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph, stream=s, **_capture_mode()):
+        with capturing(self.graph, s, **_capture_mode()):
             self.out = net.run_batch(self.states, noise=self.noise)
         self.policy = net.policy
 
