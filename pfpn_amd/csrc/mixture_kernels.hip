@@ -949,7 +949,8 @@ template <bool V> struct BoolTag { static constexpr bool value = V; };
 // visibility: `sc1` payload -> vmcnt(0) -> atomic ticket -> `sc1` loads by the wave whose add returned last).
 // The counters live in the CALLER'S workspace (its last WIDE_TICK_WORDS words, see wide_tickets()): two launches in flight on two
 // streams with two workspaces share nothing.  The entry point zeroes the counters a launch uses stream-ordered in front of it
-// (hipMemsetAsync: a memset node under capture), so a fresh (uninitialised) or poisoned workspace is repaired, not trusted.
+// (a fill kernel: memset nodes of captured graphs have given wrong results on later replays), so a fresh (uninitialised) or poisoned
+// workspace is repaired, not trusted.
 constexpr int WIDE_TICK_FWD = 0;                     // [64]   one per row chunk c (C <= 64)
 constexpr int WIDE_TICK_PPO = 64;                    // [1]    the chunks whose PPO head is done (forward + PPO head in one launch)
 constexpr int WIDE_TICK_BWD = 128;                   // [4096] one per action dim
@@ -2108,7 +2109,7 @@ size_t pfpn_mixture_workspace_bytes(int B, int A, int N) {
     const size_t AN = (size_t)A * N;
     const size_t slabs = (N <= 64 ? (size_t)1024 : (size_t)64) * (3 * AN + 4);
     // ... + the one-launch PPO pass's exchange area (pfpn_ppo_wide_fused) and, as the LAST WIDE_TICK_WORDS words, the wide
-    // kernels' hand-off tickets (wide_tickets()): adjacent, so that the fused pass zeroes both with ONE memset node
+    // kernels' hand-off tickets (wide_tickets()): adjacent, so that the fused pass zeroes both with ONE fill launch
     return (((slabs + (size_t)B * A + 64) * sizeof(float) + 15) & ~(size_t)15) + (WIDE_F2L_SYNC_WORDS + WIDE_TICK_WORDS) * sizeof(unsigned);
 }
 
@@ -2119,13 +2120,22 @@ static unsigned* wide_tickets(void* workspace, size_t workspace_bytes, int B, in
     if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 3)) return nullptr;
     return (unsigned*)((char*)workspace + need - WIDE_TICK_WORDS * sizeof(unsigned));
 }
+__global__ __launch_bounds__(256) void k_zero_words(unsigned* __restrict__ p, size_t n) {
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) p[i] = 0u;
+}
+static bool zero_words(void* p, size_t n, hipStream_t st) {
+    if (n == 0) return true;
+    const size_t blocks = (n + 255) / 256;
+    hipLaunchKernelGGL(k_zero_words, dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, st, (unsigned*)p, n);
+    return hipGetLastError() == hipSuccess;
+}
 // zero `n` tickets from `first` on, stream-ordered in front of the launch that draws them (-DPFPN_WIDE_TRUST_TICKETS, A/B build
 // knob only: rely on the last arriver having handed them back zeroed)
 static bool wide_zero_tickets(unsigned* tick, int first, int n, hipStream_t st) {
 #ifdef PFPN_WIDE_TRUST_TICKETS
     return true;
 #else
-    return hipMemsetAsync(tick + first, 0, (size_t)n * sizeof(unsigned), st) == hipSuccess;
+    return zero_words(tick + first, (size_t)n, st);
 #endif
 }
 
@@ -2300,8 +2310,8 @@ int pfpn_ppo_wide_fused(const float* logits, const float* action, const float* l
     p.clip_lo = 1.0f - clip_eps; p.clip_hi = 1.0f + clip_eps; p.value_coef = value_coef; p.inv_B = 1.0f / (float)B;
     p.dlogp = dlogp; p.dvalue = dvalue; p.loss3 = loss3;
     p.sums = sync + WIDE_F2L_PART_WORDS + WIDE_F2L_XCC_WORDS;
-    // ONE memset node: the exchange area (tags 0 = nothing published) and the tickets this launch draws
-    if (hipMemsetAsync(sync, 0, (WIDE_F2L_SYNC_WORDS + WIDE_TICK_BWD + (size_t)A) * sizeof(unsigned), st) != hipSuccess)
+    // ONE fill launch: the exchange area (tags 0 = nothing published) and the tickets this launch draws
+    if (!zero_words(sync, WIDE_F2L_SYNC_WORDS + WIDE_TICK_BWD + (size_t)A, st))
         return PFPN_ERR_LAUNCH;
     const int blocks = C * nb;
 #define PFPN_F2L_LAUNCH(SS, DD, FF)                                                                          \
@@ -2326,8 +2336,8 @@ static int logprob_bwd_impl(const float* logits, const float* x, const float* lo
     hipStream_t st = (hipStream_t)stream;
     const int AN = A * N;
     if (B == 0) {
-        (void)hipMemsetAsync(dloc, 0, AN * sizeof(float), st);
-        (void)hipMemsetAsync(dlogstd, 0, AN * sizeof(float), st);
+        (void)zero_words(dloc, AN, st);
+        (void)zero_words(dlogstd, AN, st);
         return PFPN_OK;
     }
     if (!workspace) return PFPN_ERR_WORKSPACE;
