@@ -682,7 +682,7 @@ def main():
             with torch.cuda.stream(side_):
                 shard_call()
                 torch.cuda.synchronize()
-                with torch.cuda.graph(g_, stream=side_, **graphs._capture_mode()):
+                with graphs.capturing(g_, side_, **graphs._capture_mode()):
                     for _ in range(20):
                         shard_call()
             torch.cuda.synchronize()
@@ -721,7 +721,7 @@ def main():
             with torch.cuda.stream(side_):
                 call()
                 torch.cuda.synchronize()
-                with torch.cuda.graph(g_, stream=side_, **graphs._capture_mode()):
+                with graphs.capturing(g_, side_, **graphs._capture_mode()):
                     for _ in range(per_graph):
                         call()
             torch.cuda.synchronize()
@@ -753,7 +753,7 @@ def main():
             with torch.cuda.stream(side):
                 call()
                 torch.cuda.synchronize()
-                with torch.cuda.graph(g, stream=side, **graphs._capture_mode()):
+                with graphs.capturing(g, side, **graphs._capture_mode()):
                     for _ in range(per_graph):
                         call()
             torch.cuda.synchronize()
@@ -862,7 +862,7 @@ def main():
                 with torch.cuda.stream(sideq):
                     callq()
                     torch.cuda.synchronize()
-                    with torch.cuda.graph(gqr, stream=sideq, **graphs._capture_mode()):
+                    with graphs.capturing(gqr, sideq, **graphs._capture_mode()):
                         for _ in range(10):
                             callq()
                 torch.cuda.synchronize()
