@@ -66,7 +66,8 @@ __device__ __forceinline__ double row_weight(const CatArgs& p, size_t b) {
 // row; phase 3: the gradients from the exponentials that phase 1 left in registers (IT segments a group; IT = 0, rows too wide
 // for that: from the logits again, out of the caches).
 // Bound: HBM, one read of the logits and one write of the gradient.  8192 x 128 x 256 float32: 380 us = 5.7 TB/s (a 1-GiB copy on
-// the same card: 425 us); 4096 x 36 x 35: 13.8 us = 3.0 TB/s, one wave of blocks, latency and instructions (13 us of VALU issue).
+// the same card: 425 us); 4096 x 36 x 35: 13.0 us = 3.2 TB/s, one wave of blocks: instructions issue for 5.4 us of
+// it, waves wait for half of their time.
 // What it measured on the way, 8192 x 128 x 256: reading the logits twice 933 us; holding 64 exponentials a thread, spilled around
 // the 64-bit head, 555 us; loads behind bounds branches (hipcc waits for each one) 511 us; clamped loads without a branch and half
 // of the exponentials parked in LDS 395 us.  Eight lanes x 5 for 35 particles, not 4 x 9: fewer waves, 14.1 against 16.2 us.
@@ -283,9 +284,9 @@ __global__ __launch_bounds__(NT, E * IT > 32 ? 4 : 8) void k_cat_rows(CatArgs p)
 // is formed from the registers.  For A = 1 (a token row) the loss head sits in between, run by one wave (of eight packs three wait in
 // LDS meanwhile: its 64-bit arithmetic would spill them).  64 to 1024 threads of four packs, 1024 of eight (two blocks a CU: one reads
 // while the other writes) or sixteen (one block a CU), the fewest that hold the row.
-// Bound: HBM.  6001 x 50021 bfloat16, a fifth of the rows without weight: 235 us = 4.6 TB/s (two kernels that read the logits twice:
-// 337 us); gradient of 2047 x 32001 float16: 55 us = 4.8 TB/s (86 us).  It was bound by instructions (23 an element) until the
-// exponent became one fma, the maxima packed and the join of the waves a lane each: 60 -> 55 us, 253 -> 235 us.
+// Bound: HBM.  6001 x 50021 bfloat16, a fifth of the rows without weight: 241 us = 4.5 TB/s (two kernels that read the logits twice:
+// 337 us); gradient of 2047 x 32001 float16: 55 us = 4.8 TB/s (86 us).  One fma an exponent, packed maxima and
+// the join of the waves a lane each: 60 -> 55 us, 253 -> 241 us (13 vector instructions an element now, 25 us of issue in the 55).
 // ---------------------------------------------------------------------------------------------------------------------
 template <int NW>
 __device__ __forceinline__ void block_softmax(float m, float s, float* red, float& M, float& S) {

@@ -11,7 +11,8 @@ namespace pfpn {
 
 // ---------------------------------------------------------------------------------------------------------------------
 // The same loss on log-probs that come from elsewhere (the particle mixture's own density): one pass over [n] vectors.
-// 1000003 rows, weighted: 7.6 us + 2.3 us for the sum of the blocks (24 MB: 3.7 us at the cache's rate).
+// 1000003 rows, weighted: 8.3 us + 2.3 us for the sum of the blocks (24 MB: 3.7 us at the cache's rate): latency, two waves a SIMD that
+// wait for half of their time; their instructions, the 64-bit exponential among them, issue for 3.2 us.
 // ---------------------------------------------------------------------------------------------------------------------
 // Four rows a load, from any alignment.  One block (n <= 4096) finishes the sums itself.
 constexpr long long ROWS_SMALL = 4096;

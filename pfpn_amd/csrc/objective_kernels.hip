@@ -12,8 +12,9 @@ namespace pfpn {
 //   logistic:  -(1 - e) log sigma(margin) - e log sigma(-margin)      squared:  (delta - 1 / (2 beta))^2
 // mean over the pairs;  dlogp_t = +-(d loss / d delta) w_t.  Segment sums in 64 bits: thousands of terms, and their difference.
 // Bound: HBM / cache (12-16 bytes a step) for long segments; 1500 pairs of 3000017 steps: 15.0 us + 3.8 us for the sum of the pairs =
-// 3.2 TB/s, held back by what a block does once (bounds, 64-bit sums across lanes, the head): 128 threads a pair 18.5 us, 512 15.0 us,
-// 256 15.3 us with half the waves.  Two kernels, sums and gradients, took 38 us.  24 pairs: 5.1 us, one block, one launch (was 9 us).
+// 3.2 TB/s, held back by what a block does once (bounds, 64-bit sums across lanes, the head: its instructions issue for 4.2 us of the 15,
+// waves wait for half of their time): 128 threads a pair 18.5 us, 512 15.0 us, 256 15.3 us with half the waves.  Two kernels, sums and
+// gradients, took 38 us.  24 pairs: 4.9 us, one block, one launch (was 9 us).
 // =====================================================================================================================
 struct PrefArgs {
     const float* logp;
@@ -336,10 +337,11 @@ __global__ __launch_bounds__(FINISH_NT) void k_pref_finish(const double* __restr
 //   d l[b, a, n] = coef N / (A V) p_n (f_n - sum_m f_m p_m)         (f is a count: no gradient through it)
 // k_bal_stats leaves sums and counts of every chunk of rows as slabs, k_bal_reduce adds the slabs (64 bits, in order), k_bal_grad
 // writes the gradient.  A group of G lanes keeps ONE choice a while it walks rows: its sums, and f, stay in registers.
-// Bound: k_bal_stats instructions (the K-th largest), k_bal_grad HBM, k_bal_reduce latency.  262147 x 128 bfloat16, top 8, masked: 50 + 5 +
-// 32 us (two readings and a writing of 67 MB: 40 us); 4096 x 36 x 35 float32, top 1: 11.0 + 5.2 + 9.7 us (20 MB: 6.4 us, three launches).
+// Bound: k_bal_stats instructions (the K-th largest: issue 31 of its 44 us), k_bal_grad HBM, k_bal_reduce latency.  262147 x 128 bfloat16,
+// top 8, masked: 44 + 5 + 29 us (two readings and a writing of 67 MB: 40 us); 4096 x 36 x 35 float32, top 1: 10.8 + 5.2 + 9.8 us (20 MB:
+// 6.4 us; three launches, each of them issue for half of its time and waiting for the other).
 // Top 8 of 128 on the way: eight rounds of the group's maximum 117 us, rounds on sorted lists 74 us, joined lists of eight 66 us, keys that
-// hold the index (no ranking of equal logits afterwards) 57 us, 256 instead of 512 chunks of rows 49 us.
+// hold the index (no ranking of equal logits afterwards) 57 us, 256 instead of 512 chunks of rows 49 us, eight waves a block for nine 44 us.
 // =====================================================================================================================
 struct BalArgs {
     const void* logits;
