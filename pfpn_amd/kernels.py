@@ -12,7 +12,7 @@ import torch
 
 from . import _lib
 
-_ws = {}
+_ws, _ws_outgrown = {}, []
 
 
 def _stream():
@@ -34,11 +34,15 @@ def _f32(t, *shape, name="tensor"):
 
 def workspace(nbytes, device):
     """Grow-only per-device scratch buffer (never reallocated inside a captured region if it was
-    sized by a warm-up call first)."""
+    sized by a warm-up call first).  A buffer that was outgrown stays allocated: torch hands its streams out again in turn, and a
+    step captured on one earlier goes on writing there.  (Each is at least twice the one before: together less than the latest.)"""
     # one buffer per (device, stream): kernels on a side stream must not share slabs with the main stream
     key = (device.index if device.index is not None else torch.cuda.current_device(), _stream())
     buf = _ws.get(key)
     if buf is None or buf.numel() < nbytes:
+        if buf is not None:
+            _ws_outgrown.append(buf)
+            nbytes = max(int(nbytes), 2 * buf.numel())
         buf = torch.empty(int(nbytes), dtype=torch.uint8, device=device)
         _ws[key] = buf
     return buf

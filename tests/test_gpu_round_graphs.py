@@ -141,3 +141,18 @@ def test_nothing_is_collected_inside_a_capture(dev, monkeypatch, what):
     gc.collect()
     assert len(_Garbage.seen) > 100 and not any(_Garbage.seen)
     assert g is not None
+
+
+def test_an_outgrown_workspace_is_not_handed_out_again(dev):
+    """a captured step holds the address of the scratch buffer it was captured with: when a larger size replaces the buffer of that
+    stream, its memory must not become another tensor's"""
+    from pfpn_amd import kernels
+    with torch.cuda.stream(torch.cuda.Stream()):
+        first = kernels.workspace(3 << 20, dev)
+        lo, hi = first.data_ptr(), first.data_ptr() + first.numel()
+        del first
+        second = kernels.workspace(hi - lo + 1, dev)
+        assert second.data_ptr() != lo and second.numel() >= 2 * (hi - lo)
+        assert kernels.workspace(1000, dev).data_ptr() == second.data_ptr()
+        others = [torch.empty(3 << 20, dtype=torch.uint8, device=dev) for _ in range(20)]
+        assert all(t.data_ptr() >= hi or t.data_ptr() + t.numel() <= lo for t in others)
