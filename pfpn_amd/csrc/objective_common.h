@@ -304,7 +304,7 @@ __device__ __forceinline__ double kl_sample(double d, double& em1) {
 __device__ __forceinline__ double policy_head(double logp, const HeadRow& row, const HeadArgs& h, HeadTerms& t) {
     const double r = exp(logp - (double)row.logp_old), a = (double)row.a;
     const double held_r = r < h.clip_lo ? h.clip_lo : (r > h.clip_hi ? h.clip_hi : r);
-    const double sur = a == 0.0 && r > h.clip_hi ? 0.0 : r * a;        // (no advantage, no surrogate: not inf * 0)
+    const double sur = a == 0.0 && r > 1.0 ? 0.0 : r * a;              // (no advantage, no surrogate: not inf * 0)
     const double held = held_r * a;
     const bool clipped = held < sur;
     double g = clipped ? 0.0 : -sur;

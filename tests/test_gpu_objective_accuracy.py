@@ -128,6 +128,14 @@ def test_far_log_probs(dev):
     assert d[0].isnan() and d[1] == 0 and l4[0].isnan()
 
 
+def test_rows_without_advantage_under_a_one_sided_clip(dev):
+    """no upper bound on the ratio, an impossible old choice, no advantage: nothing, not inf * 0"""
+    from pfpn_amd import kernels
+    old, adv = torch.tensor([-math.inf, -2000.0, -1.0, -1.0], device=dev), torch.tensor([0.0, 0.0, 0.0, 2.0], device=dev)
+    d, l4 = kernels.policy_kl_loss(torch.full((4,), -1.0, device=dev), old, adv, clip_eps=(0.2, math.inf))
+    assert d.tolist() == [0.0, 0.0, 0.0, -0.5] and l4.tolist() == [-0.5, -0.5, 0.0, 0.0]
+
+
 @pytest.mark.parametrize("shape", [(36, 40, 8), (36, 2, 300), (36, 1, 5000), (600, 1, 1500), (5, 3, 1100), (3, 1, 70001)])
 def test_far_log_probs_from_logits(dev, shape):
     from pfpn_amd import kernels
